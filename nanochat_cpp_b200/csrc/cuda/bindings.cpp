@@ -141,6 +141,7 @@ void register_optim(pybind11::module_& m);
 void register_comm(pybind11::module_& m);
 void register_decode(pybind11::module_& m);
 void register_fp8(pybind11::module_& m);
+void register_serving(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", &gemm, "tcgen05 bf16 GEMM with fused epilogue", pybind11::arg("A"), pybind11::arg("B"),
@@ -170,5 +171,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 #endif
 #ifdef NC_HAVE_FP8
   register_fp8(m);
+#endif
+#ifdef NC_HAVE_SERVING
+  register_serving(m);
 #endif
 }

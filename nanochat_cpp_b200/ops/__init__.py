@@ -123,6 +123,7 @@ _NAMES = [
     "attention_fwd", "attention_bwd", "value_gate_fwd", "value_gate_bwd", "smear_fwd", "smear_bwd",
     "embedding_fwd", "embedding_bwd", "embedding_order", "classifier_fwd_bwd", "adamw_update", "muon_update",
     "grad_norm_and_clip", "kv_append", "paged_decode_attention", "quantize_fp8", "gemm_scaled_fp8",
+    "kv_append_mx", "kv_read_mx", "paged_decode_attention_mx", "paged_chunk_attention", "sample_rows",
 ]
 for _n in _NAMES:
     globals()[_n] = _dispatch(_n)

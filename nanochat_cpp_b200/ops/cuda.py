@@ -486,6 +486,40 @@ def paged_decode_attention(q, k_pool, v_pool, page_table, seq_lens, window_left=
     return _C.paged_decode_attention(q, k_pool, v_pool, page_table, seq_lens, int(window_left), float(scale))
 
 
+# ---------------------------------------------------------------------------
+# MXFP8 KV cache, attention of new tokens over the pages, sampling
+# ---------------------------------------------------------------------------
+def kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new):
+    _C.kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new)
+
+
+def kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions):
+    k, v = _C.kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions)
+    return k, v
+
+
+def paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left=-1, scale=None):
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    return _C.paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left, scale)
+
+
+def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, window_left=-1, scale=None,
+                          k_scale=None, v_scale=None):
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    return _C.paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale)
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    rows = [x if isinstance(x, torch.Tensor) else None for x in (temperature, top_k, top_p, min_p)]
+    if rows == [None, None, None, None]:
+        return _C.sample_rows(logits, u, temperature, top_k, top_p, min_p, None, None, None, None)
+    t, k, tp, mp = (d if r is not None else x for x, r, d in
+                    zip((temperature, top_k, top_p, min_p), rows, (1.0, 0, 1.0, 0.0)))
+    return _C.sample_rows(logits, u, t, k, tp, mp, *rows)
+
+
 def __getattr__(name):
     # Operators without a kernel are an error on a GPU, not a fallback.
     raise AttributeError(f"ops.cuda has no operator {name!r}")

@@ -609,3 +609,218 @@ def paged_decode_attention(q, k_pool, v_pool, page_table, seq_lens, window_left=
     s = s.masked_fill(~ok[:, None, :], float("-inf"))
     p = torch.softmax(s, dim=-1)
     return torch.einsum("bhs,bshd->bhd", p, v).to(q.dtype)
+
+
+# --------------------------------------------------------------------------
+# MXFP8 KV cache. Code pools are uint8 [num_pages, page_size, KV, D] (E4M3), scale pools uint8
+# [num_pages, KV, page_size, D / 32]: one biased power-of-two exponent per token, head and 32 channels
+# --------------------------------------------------------------------------
+def _check(ok, msg):
+    if not ok:
+        raise ValueError(msg)
+
+
+def _check_mx_pools(name, k_pool, v_pool, k_scale, v_scale):
+    _check(k_pool.dim() == 4 and k_pool.dtype == torch.uint8 and k_pool.is_contiguous(),
+           f"{name}: k_pool must be contiguous uint8 [pages, page_size, KV, D]")
+    _check(v_pool.shape == k_pool.shape and v_pool.dtype == torch.uint8 and v_pool.is_contiguous(),
+           f"{name}: v_pool must have the shape and type of k_pool")
+    P, page, KV, D = k_pool.shape
+    _check(D in (64, 128), f"{name}: head_dim must be 64 or 128")
+    _check(page > 0 and KV > 0, f"{name}: page_size and kv heads must be positive")
+    for s in (k_scale, v_scale):
+        _check(s is not None and s.dtype == torch.uint8 and tuple(s.shape) == (P, KV, page, D // 32) and s.is_contiguous(),
+               f"{name}: scales must be contiguous uint8 [pages, KV, page_size, D / 32]")
+
+
+def _check_table(name, page_table, B):
+    _check(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous() and
+           page_table.shape[0] == B and page_table.shape[1] > 0, f"{name}: page_table must be contiguous int32 [B, max_pages]")
+
+
+def mx_kv_encode(x):
+    """[..., D] -> (codes uint8 [..., D], scale bytes uint8 [..., D / 32]): `quantize_fp8` of every row, with one
+    addition: a block that holds a NaN is NaN as a whole (scale byte 255, every code 0x7f)."""
+    from .fp8 import ref_mx_quantize
+    D = x.shape[-1]
+    q, eb = ref_mx_quantize(x.reshape(-1, D).to(torch.bfloat16))
+    q = q.view(torch.uint8).view(-1, D // 32, 32)
+    bad = x.reshape(-1, D // 32, 32).isnan().any(-1)
+    q = torch.where(bad[..., None], torch.full_like(q, 0x7F), q)
+    eb = torch.where(bad, torch.full_like(eb, 255), eb)
+    return q.view(x.shape), eb.view(*x.shape[:-1], D // 32)
+
+
+def mx_kv_decode(codes, scale):
+    """fp32 values of codes [..., D] with scale bytes [..., D / 32]."""
+    D = codes.shape[-1]
+    v = codes.view(torch.float8_e4m3fn).float().reshape(*codes.shape[:-1], D // 32, 32)
+    return (v * torch.exp2(scale.float() - 127.0)[..., None]).reshape(codes.shape)
+
+
+def _page_slots(pool, page_table, positions):
+    """(usable [B, T], page [B, T], slot [B, T]) of absolute positions; unusable: negative, past the table, or on a
+    page outside the pool."""
+    page_size, n = pool.shape[1], page_table.shape[1]
+    pos = positions.long()
+    inside = (pos >= 0) & (pos < n * page_size)
+    at = torch.where(inside, pos, torch.zeros_like(pos))
+    page = torch.gather(page_table.long(), 1, at // page_size)
+    ok = inside & (page >= 0) & (page < pool.shape[0])
+    return ok, torch.where(ok, page, torch.zeros_like(page)), at % page_size
+
+
+def _check_rows(name, x, positions, k_pool):
+    _check(x.dim() == 4 and tuple(x.shape) == (*positions.shape, *k_pool.shape[2:]) and x.stride(3) == 1,
+           f"{name}: new rows must be [B, T, KV, D] with dense channels")
+
+
+def kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new):
+    """Quantise rows k_new / v_new [B, T, KV, D] (bf16) to MXFP8 and write them at absolute positions `positions`
+    [B, T] (int32; < 0 = skip) of their sequences' pages. Positions of one sequence that are not negative must differ."""
+    name = "kv_append_mx"
+    _check_mx_pools(name, k_pool, v_pool, k_scale, v_scale)
+    _check(positions.dtype == torch.int32 and positions.dim() == 2 and positions.is_contiguous(),
+           f"{name}: positions must be contiguous int32 [B, T]")
+    _check_table(name, page_table, positions.shape[0])
+    _check_rows(name, k_new, positions, k_pool)
+    _check_rows(name, v_new, positions, k_pool)
+    if positions.numel() == 0:
+        return
+    ok, page, slot = _page_slots(k_pool, page_table, positions)
+    for pool, scale, new in ((k_pool, k_scale, k_new), (v_pool, v_scale, v_new)):
+        codes, eb = mx_kv_encode(new)
+        pool[page[ok], slot[ok]] = codes[ok]
+        scale[page[ok], :, slot[ok]] = eb[ok]
+
+
+def kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions):
+    """Rows of an MXFP8 cache as the bf16 values they stand for: (k, v), each [B, T, KV, D], at absolute positions
+    `positions` [B, T] (int32). A negative position gives a row of zeros."""
+    name = "kv_read_mx"
+    _check_mx_pools(name, k_pool, v_pool, k_scale, v_scale)
+    _check(positions.dtype == torch.int32 and positions.dim() == 2 and positions.is_contiguous(),
+           f"{name}: positions must be contiguous int32 [B, T]")
+    _check_table(name, page_table, positions.shape[0])
+    ok, page, slot = _page_slots(k_pool, page_table, positions)
+    out = []
+    for pool, scale in ((k_pool, k_scale), (v_pool, v_scale)):
+        row = mx_kv_decode(pool[page, slot], scale[page, :, slot])
+        out.append(torch.where(ok[..., None, None], row, torch.zeros_like(row)).to(torch.bfloat16))
+    return out[0], out[1]
+
+
+def _paged_chunk(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale):
+    """One sequence at a time: queries t < q_lens[b] at positions seq_lens[b] - q_lens[b] + t."""
+    B, T, H, D = q.shape
+    KV = k_pool.shape[2]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    acc = _acc(q)
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    for b in range(B):
+        L = int(seq_lens[b])
+        n = T if q_lens is None else min(max(int(q_lens[b]), 0), T)
+        S = min(L, page_table.shape[1] * k_pool.shape[1])
+        if n <= 0 or S <= 0:
+            continue
+        j = torch.arange(S, dtype=torch.int32, device=q.device)[None, :]
+        ok, page, slot = _page_slots(k_pool, page_table[b:b + 1], j)
+        k, v = k_pool[page[0], slot[0]], v_pool[page[0], slot[0]]
+        if k_scale is not None:
+            k, v = mx_kv_decode(k, k_scale[page[0], :, slot[0]]), mx_kv_decode(v, v_scale[page[0], :, slot[0]])
+        qpos = torch.arange(L - n, L, device=q.device)[:, None]
+        seen = (j <= qpos) & ok
+        if window_left is not None and window_left >= 0:
+            seen = seen & (qpos - j <= window_left)
+        used = seen.any(0)                         # a key that no query sees is not read at all
+        seen, k, v = seen[:, used], k[used].to(acc), v[used].to(acc)
+        if not used.any():
+            continue
+        k, v = k.repeat_interleave(H // KV, dim=1), v.repeat_interleave(H // KV, dim=1)
+        s = torch.einsum("thd,shd->hts", q[b, :n].to(acc), k) * scale
+        s = s.masked_fill(~seen[None], float("-inf"))
+        p = torch.where(seen.any(1)[None, :, None], torch.softmax(s, dim=-1), torch.zeros_like(s))
+        out[b, :n] = torch.einsum("hts,shd->thd", p, v).to(q.dtype)
+    return out
+
+
+def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, window_left=-1, scale=None,
+                          k_scale=None, v_scale=None):
+    """Attention of a chunk of new tokens over the paged cache, their own keys included (append first). q [B, T, H, D];
+    the first q_lens[b] (None: T) rows of sequence b are its last q_lens[b] positions of seq_lens[b]. Row t sees keys
+    j <= its position p = seq_lens[b] - q_lens[b] + t with p - j <= window_left. With `k_scale` / `v_scale` the pools
+    are MXFP8 (see `kv_append_mx`), without them they have the type of q. Rows at or behind q_lens[b] and rows that
+    see no key are zero. A key past the page table or on a page outside the pool is left out."""
+    name = "paged_chunk_attention"
+    _check(q.dim() == 4 and q.stride(3) == 1 and q.shape[3] in (64, 128), f"{name}: q must be [B, T, H, D], D 64 or 128")
+    B, T, H, D = q.shape
+    _check((k_scale is None) == (v_scale is None), f"{name}: give both scales or neither")
+    if k_scale is not None:
+        _check_mx_pools(name, k_pool, v_pool, k_scale, v_scale)
+    else:
+        _check(k_pool.dim() == 4 and k_pool.dtype == q.dtype and k_pool.is_contiguous() and v_pool.shape == k_pool.shape and
+               v_pool.dtype == q.dtype and v_pool.is_contiguous(),
+               f"{name}: pools must be contiguous [pages, page_size, KV, D] of q's type")
+    _check(k_pool.shape[3] == D and H % k_pool.shape[2] == 0, f"{name}: heads must be a multiple of kv heads, one head_dim")
+    _check_table(name, page_table, B)
+    for x in (seq_lens, q_lens):
+        _check(x is None or (x.dtype == torch.int32 and tuple(x.shape) == (B,) and x.is_contiguous()),
+               f"{name}: seq_lens and q_lens must be contiguous int32 [B]")
+    return _paged_chunk(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale)
+
+
+def paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left=-1, scale=None):
+    """`paged_decode_attention` over an MXFP8 cache (see `kv_append_mx`): one query per sequence, q [B, H, D], at
+    position seq_lens[b] - 1. A sequence of no tokens gives a row of zeros."""
+    _check(q.dim() == 3, "paged_decode_attention_mx: q must be [B, H, D]")
+    return paged_chunk_attention(q[:, None], k_pool, v_pool, page_table, seq_lens, None, window_left, scale,
+                                 k_scale, v_scale)[:, 0]
+
+
+# --------------------------------------------------------------------------
+# Sampling from given random numbers
+# --------------------------------------------------------------------------
+def _per_row(name, x, R, dtype, device):
+    if isinstance(x, torch.Tensor):
+        _check(x.dtype == dtype and tuple(x.shape) == (R,) and x.is_contiguous(),
+               f"sample_rows: {name} must be a number or a contiguous {dtype} [rows] tensor")
+        return x.to(device)[:, None]
+    return torch.full((R, 1), x, dtype=dtype, device=device)
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of logits [R, V] (bf16 or fp32) from the random numbers u [R] (fp32, in [0, 1)): int64 [R].
+
+    p_i = exp((z_i - max z) / temperature). Kept are, in this order: the top_k largest (<= 0: all), those with p_i >= min_p,
+    and of these, in descending order, the shortest run whose mass reaches top_p of theirs (>= 1: all; the largest is always
+    kept). Among equal logits the lowest index comes first. The token is the first kept index, in vocabulary order, at
+    which the running mass exceeds u times the kept mass. temperature <= 0 takes the largest logit. Each setting is a
+    number or a tensor with one value per row (fp32; top_k int32). NaN counts as -inf; a row without a value above
+    -inf gives -1. Masses are summed in 64 bits."""
+    _check(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[1] > 0 and
+           logits.stride(1) == 1, "sample_rows: logits must be bf16 or fp32 [rows, vocab] with dense rows")
+    R, V = logits.shape
+    _check(u.dtype == torch.float32 and tuple(u.shape) == (R,) and u.is_contiguous(), "sample_rows: u must be contiguous fp32 [rows]")
+    dev = logits.device
+    t = _per_row("temperature", temperature, R, torch.float32, dev).double()
+    k = _per_row("top_k", top_k, R, torch.int32, dev)
+    tp = _per_row("top_p", top_p, R, torch.float32, dev).double()
+    mp = _per_row("min_p", min_p, R, torch.float32, dev).double()
+    if R == 0:
+        return torch.empty(0, dtype=torch.int64, device=dev)
+    z = logits.double()
+    z = torch.where(z.isnan(), torch.full_like(z, float("-inf")), z)
+    z, order = z.sort(dim=1, descending=True, stable=True)
+    top = z[:, :1]
+    x = torch.where(z == top, torch.zeros_like(z), (z - top) / torch.where(t > 0, t, torch.ones_like(t)))
+    p = torch.where(z == float("-inf"), torch.zeros_like(z), torch.exp(x))
+    rank = torch.arange(V, device=dev)[None, :]
+    p = torch.where(((rank < k) | (k <= 0)) & (p >= mp) | (rank == 0), p, torch.zeros_like(p))
+    before = p.cumsum(1) - p
+    p = torch.where((tp >= 1) | (before < tp * p.sum(1, keepdim=True)) | (rank == 0), p, torch.zeros_like(p))
+    p = torch.where((t > 0) | (rank == 0), p, torch.zeros_like(p))
+    cum = torch.zeros_like(p).scatter_(1, order, p).cumsum(1)
+    token = (cum <= u.double()[:, None] * cum[:, -1:]).sum(1)
+    last = (cum < cum[:, -1:]).sum(1)          # the first index at which all the mass is reached
+    token = torch.minimum(token, last)
+    return torch.where(top[:, 0] == float("-inf"), torch.full_like(token, -1), token)
