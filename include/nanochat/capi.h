@@ -251,6 +251,7 @@ int64_t ncb_parquet_read(const char* path, const char* column, char* bytes, int6
  * [rows, vocab] fp32 (soft-capped). Greedy when temperature <= 0. */
 void ncb_sample_rows(const float* logits, int rows, int vocab, float temperature, int top_k, uint64_t seed,
                      const int64_t* row_ids, int64_t draw_index, int* out);
+void ncb_sample_uniforms(uint64_t seed, const int64_t* row_ids, int rows, int64_t first_draw, int draws, float* out);
 int ncb_sample_token(const float* logits, int vocab, float temperature, int top_k, uint64_t seed, uint64_t row,
                      uint64_t step);
 

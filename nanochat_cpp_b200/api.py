@@ -216,13 +216,15 @@ class Model:
         load_checkpoint(os.fspath(path), self.gpt)
 
     def generate(self, prompt, max_tokens: int = 256, temperature: float = 1.0, top_k: int = 0, seed: int = 0,
-                 num_samples: int = 1, stop_id: int = -1, bos_id: int = -1) -> List[GeneratedRow]:
+                 num_samples: int = 1, stop_id: int = -1, bos_id: int = -1, top_p: float = 1.0, min_p: float = 0.0,
+                 kv_cache: str = "auto") -> List[GeneratedRow]:
         from .inference import GenerateParams, InferenceEngine, generate
-        if not hasattr(self, "_engine"):
-            self._engine = InferenceEngine(self.gpt)
+        if not hasattr(self, "_engine") or self._engine.kv_dtype != kv_cache:
+            self._engine = InferenceEngine(self.gpt, kv_dtype=kv_cache)
         rows = generate(self._engine, list(prompt), GenerateParams(num_samples=num_samples, max_tokens=max_tokens,
                                                                    temperature=temperature, top_k=top_k, seed=seed,
-                                                                   stop_id=stop_id, bos_id=bos_id))
+                                                                   stop_id=stop_id, bos_id=bos_id, top_p=top_p,
+                                                                   min_p=min_p))
         return [GeneratedRow(r.tokens, r.mask) for r in rows]
 
     def no_grad(self):

@@ -270,6 +270,9 @@ def _generate_parser(sub):
     ap.add_argument("--num-samples", type=int, default=1)
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0, help="nucleus sampling (on the device)")
+    ap.add_argument("--min-p", type=float, default=0.0, help="least probability kept, relative to the largest (on the device)")
+    ap.add_argument("--kv-cache", choices=("auto", "mxfp8"), default="auto", help="what cached keys and values are stored as")
     ap.add_argument("--stop-id", type=int, default=-1)
     ap.add_argument("--bos-id", type=int, default=-1)
     ap.add_argument("--seed", type=int, default=0)
@@ -301,9 +304,9 @@ def cmd_generate(a) -> int:
     if not prompts:
         print("generate: no prompt (--prompt, --text-file, --tokens or --prompt-file)", file=sys.stderr)
         return 2
-    eng = InferenceEngine(model)
+    eng = InferenceEngine(model, kv_dtype=a.kv_cache)
     params = GenerateParams(num_samples=a.num_samples, max_tokens=a.max_tokens, temperature=a.temperature,
-                            top_k=a.top_k, seed=a.seed, stop_id=a.stop_id, bos_id=a.bos_id)
+                            top_k=a.top_k, seed=a.seed, stop_id=a.stop_id, bos_id=a.bos_id, top_p=a.top_p, min_p=a.min_p)
     rows = []
     by_len = {}
     for i, p in enumerate(prompts):                # prompts of one length decode as one batch

@@ -587,6 +587,18 @@ void ncb_sample_rows(const float* logits, int rows, int vocab, float temperature
   }
 }
 
+// The numbers in [0, 1) that those streams draw, for samplers that run elsewhere: out[d * rows + r] is draw
+// `first_draw + d` of row `row_ids[r]`, the value that ncb_sample_rows compares with the running mass.
+void ncb_sample_uniforms(uint64_t seed, const int64_t* row_ids, int rows, int64_t first_draw, int draws, float* out) {
+  if (out == nullptr || rows <= 0 || draws <= 0) return;
+  for (int r = 0; r < rows; ++r) {
+    ncb::Rng rng(ncb::MixSeed(seed, static_cast<uint64_t>(row_ids != nullptr ? row_ids[r] : r)));
+    for (int64_t k = 0; k < first_draw; ++k) rng.NextU64();
+    for (int d = 0; d < draws; ++d)
+      out[static_cast<std::size_t>(d) * rows + r] = static_cast<float>(rng.NextU64() >> 40) * 0x1p-24f;
+  }
+}
+
 int ncb_sample_token(const float* logits, int vocab, float temperature, int top_k, uint64_t seed, uint64_t row,
                      uint64_t step) {
   ncb::Rng rng(ncb::MixSeed(ncb::MixSeed(seed, row), step));

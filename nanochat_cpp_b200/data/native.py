@@ -82,6 +82,8 @@ def lib():
         L.ncb_parquet_read.restype = C.c_int64
         L.ncb_parquet_read.argtypes = [C.c_char_p, C.c_char_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
                                        C.POINTER(C.c_int64)]
+        L.ncb_sample_uniforms.restype = None
+        L.ncb_sample_uniforms.argtypes = [C.c_uint64, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p]
         L.ncb_sample_token.argtypes = [C.c_void_p, C.c_int, C.c_float, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64]
         _lib = L
     return _lib
@@ -346,6 +348,15 @@ def read_parquet_strings(path: str, column: str = "text") -> List[bytes]:
                            C.byref(total))
     raw = buf.tobytes()
     return [raw[int(offs[i]):int(offs[i + 1])] for i in range(n)]
+
+
+def sample_uniforms(seed: int, rows, first_draw: int, draws: int) -> np.ndarray:
+    """fp32 [draws, rows] in [0, 1): the numbers that the sampling stream of each row draws from `first_draw` on."""
+    ids = np.ascontiguousarray(rows, dtype=np.int64)
+    out = np.empty((draws, ids.size), dtype=np.float32)
+    lib().ncb_sample_uniforms(C.c_uint64(int(seed) & 0xFFFFFFFFFFFFFFFF), ids.ctypes.data, ids.size, int(first_draw),
+                              int(draws), out.ctypes.data)
+    return out
 
 
 def sample_token(logits: np.ndarray, temperature: float, top_k: int, seed: int, row: int = 0, step: int = 0) -> int:

@@ -22,6 +22,7 @@ from ..config import LOGIT_SOFTCAP, Config
 from ..models.gpt import GPT, _heads
 
 PAGE_SIZE = 16
+KV_DTYPES = ("auto", "mxfp8")    # auto: the model's compute dtype
 
 
 class PageAllocator:
@@ -99,7 +100,12 @@ class PagedKVCache:
     The reference's cache is one contiguous [max_seq] buffer per layer and sequence (src/generate.cc:266-300)."""
 
     def __init__(self, cfg: Config, batch: int, max_seq: int, device, dtype, page_size: int = PAGE_SIZE,
-                 pool_pages: Optional[int] = None, windowed: bool = True):
+                 pool_pages: Optional[int] = None, windowed: bool = True, kv_dtype: str = "auto"):
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {KV_DTYPES}")
+        if kv_dtype == "mxfp8" and cfg.head_dim not in (64, 128):
+            raise ValueError("an MXFP8 cache needs head_dim 64 or 128")
+        self.kv_dtype = kv_dtype
         self.cfg, self.batch, self.max_seq, self.page_size = cfg, batch, max_seq, page_size
         device = torch.device(device)
         self.pages_per_seq = (max_seq + page_size - 1) // page_size
@@ -110,16 +116,35 @@ class PagedKVCache:
         n_full = batch * self.pages_per_seq if pool_pages is None else int(pool_pages)
         # a window of w keys back plus the query touches at most (w + page) // page + 1 pages. A chunk of a long
         # prompt needs the window before its first token and stores the window before its last: twice that.
-        s_pages = min(self.pages_per_seq, 2 * ((max(self.window, 0) + page_size) // page_size + 1))
+        s_pages = 2 * ((max(self.window, 0) + page_size) // page_size + 1)
+        # `extend` writes a whole chunk before it attends, so a chunk and the window before its first token are
+        # mapped at once: chunks of a window's length fit the pages above; an MXFP8 cache, whose prompts go through
+        # `extend` as well, is given room for chunks of at least 512 tokens.
+        self.chunk = max_seq
+        if self.window >= 0:
+            self.chunk = max(self.window, 1)
+            if kv_dtype == "mxfp8":
+                self.chunk = max(self.chunk, 512)
+                s_pages = max(s_pages, (self.window + self.chunk - 1) // page_size + 2)
+        s_pages = min(self.pages_per_seq, s_pages)
         n_win = batch * s_pages
         self.full = _PageMap(batch, self.pages_per_seq, n_full, device)
         self.win = _PageMap(batch, self.pages_per_seq, n_win, device) if any(self.is_windowed) else None
         self.k, self.v = [], []
+        self.k_scale = self.v_scale = None     # MXFP8: one uint8 tensor [pages, KV, page, D / 32] per layer
+        if kv_dtype == "mxfp8":
+            dtype_kv, self.k_scale, self.v_scale = torch.uint8, [], []
+        else:
+            dtype_kv = dtype
         for i in range(cfg.num_layers):
             n = n_win if self.is_windowed[i] else n_full
             shape = (n, page_size, cfg.num_kv_heads, cfg.head_dim)
-            self.k.append(torch.zeros(shape, dtype=dtype, device=device))
-            self.v.append(torch.zeros(shape, dtype=dtype, device=device))
+            if kv_dtype == "mxfp8":
+                for scales in (self.k_scale, self.v_scale):
+                    scales.append(torch.full((n, cfg.num_kv_heads, page_size, cfg.head_dim // 32), 127, dtype=torch.uint8,
+                                             device=device))
+            self.k.append(torch.zeros(shape, dtype=dtype_kv, device=device))
+            self.v.append(torch.zeros(shape, dtype=dtype_kv, device=device))
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.lens_host = [0] * batch          # the host's copy of seq_lens (every step advances it without a sync)
         self.prev_emb = torch.zeros(batch, cfg.hidden_dim, dtype=dtype, device=device)
@@ -161,6 +186,50 @@ class PagedKVCache:
         if self.win is not None:
             self.win.push()
 
+    def prepare_chunk(self, counts: Sequence[int]) -> None:
+        """Map every page that the next counts[r] <= `chunk` tokens of sequence r are written to, on all layers, and
+        release the windowed pages that its first new query no longer sees."""
+        ps = self.page_size
+        if max(counts) > self.chunk:
+            raise ValueError("a chunk is longer than the cache's windowed layers hold at once")
+        for r, count in enumerate(counts):
+            n0 = self.lens_host[r]
+            if count < 0 or n0 + count > self.max_seq:
+                raise ValueError("sequence does not fit the KV cache")
+            if count == 0:
+                continue
+            self.full.ensure(r, n0 // ps, (n0 + count - 1) // ps)
+            if self.win is not None:
+                floor = self.append_floor(n0 + 1)
+                self.win.release_below(r, floor // ps)
+                self.win.ensure(r, n0 // ps, (n0 + count - 1) // ps)
+        self.full.push()
+        if self.win is not None:
+            self.win.push()
+
+    def append(self, layer: int, positions: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Write rows k / v [B, T, KV, D] of `layer` at absolute positions [B, T] (negative: skipped)."""
+        if self.k_scale is not None:
+            ops.kv_append_mx(self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], self.table(layer),
+                             positions, k, v)
+        else:
+            ops.kv_append(self.k[layer], self.v[layer], self.table(layer), positions, k, v)
+
+    def read(self, layer: int, row: int):
+        """The cached keys and values of one sequence as numbers: (k, v), each [length, KV, D]; zero where a windowed layer
+        has given the page back."""
+        n, ps = self.lens_host[row], self.page_size
+        table = self.table(layer)[row:row + 1].contiguous()
+        pos = torch.arange(n, dtype=torch.int32, device=table.device)[None]
+        held = torch.gather(table, 1, pos.long() // ps) >= 0
+        if self.k_scale is not None:
+            k, v = ops.kv_read_mx(self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], table,
+                                  torch.where(held, pos, torch.full_like(pos, -1)))
+            return k[0], v[0]
+        keep = held[0, :, None, None]
+        return tuple(torch.where(keep, g, torch.zeros_like(g))
+                     for g in (ops.paged_gather(p, table, n)[0] for p in (self.k[layer], self.v[layer])))
+
     def advance_host(self, count: int, rows: Optional[Sequence[int]] = None) -> None:
         for r in (range(self.batch) if rows is None else rows):
             self.lens_host[r] += count
@@ -188,7 +257,8 @@ class PagedKVCache:
         return out
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.k + self.v)
+        scales = (self.k_scale or []) + (self.v_scale or [])
+        return sum(t.numel() * t.element_size() for t in self.k + self.v + scales)
 
     def rows(self, index: Sequence[int]) -> "_CacheRows":
         return _CacheRows(self, list(index))
@@ -205,6 +275,7 @@ class _CacheRows:
         self._idx = torch.as_tensor(index, dtype=torch.long, device=dev)
         self.cfg, self.max_seq, self.page_size, self.batch = parent.cfg, parent.max_seq, parent.page_size, len(index)
         self.k, self.v = parent.k, parent.v
+        self.k_scale, self.v_scale, self.kv_dtype = parent.k_scale, parent.v_scale, parent.kv_dtype
         self.is_windowed, self.window = parent.is_windowed, parent.window
         self.seq_lens = parent.seq_lens[self._idx].clone()
         self.lens_host = [parent.lens_host[r] for r in index]
@@ -237,8 +308,13 @@ class _CacheRows:
 
 
 class InferenceEngine:
-    def __init__(self, model: GPT, use_cuda_graph: bool = True):
+    def __init__(self, model: GPT, use_cuda_graph: bool = True, kv_dtype: str = "auto"):
+        """`kv_dtype`: what `new_cache` stores keys and values as: "auto" (the model's dtype) or "mxfp8" (8 bits and a
+        shared scale per 32 channels: half the memory and traffic of bf16)."""
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {KV_DTYPES}")
         self.model = model
+        self.kv_dtype = kv_dtype
         self.cfg = model.cfg
         self.device = model.device
         self.dtype = model.dtype
@@ -251,7 +327,7 @@ class InferenceEngine:
 
     # ------------------------------------------------------------------ helpers
     def new_cache(self, batch: int, max_seq: int) -> PagedKVCache:
-        return PagedKVCache(self.cfg, batch, max_seq, self.device, self.dtype)
+        return PagedKVCache(self.cfg, batch, max_seq, self.device, self.dtype, kv_dtype=self.kv_dtype)
 
     def _rope(self, upto: int):
         if upto > self._rope_len:
@@ -293,6 +369,9 @@ class InferenceEngine:
             cos_all, sin_all = self._rope(t0 + T)
             cos, sin = cos_all[t0:t0 + T], sin_all[t0:t0 + T]
         new_lens = cache.seq_lens + T
+        mx = cache.k_scale is not None
+        if mx and not decode:
+            raise ValueError("prompts of an MXFP8 cache go through extend")
         fused_prologue = kernel_decode and D == 128 and cache.page_table.shape[0] == B
         pos_flat = pos.reshape(-1).contiguous()
         # windowed layers keep only what a later query can still see: earlier positions of a long prompt are not stored
@@ -322,7 +401,7 @@ class InferenceEngine:
                     ve = ops.embedding_fwd(tok, P.v(f"value_embeds.{i}.weight"))
                     v, _ = ops.value_gate_fwd(h, ve, m._w(i, "attn.ve_gate"), v, D)
             wl = cfg.window_left(i)
-            if fused_prologue and wqkv is not None:
+            if fused_prologue and wqkv is not None and not mx:
                 # one launch: q / k preparation, k and v appended to their pages; q comes back dense
                 table = cache.table(i)
                 q3 = ops.cuda_module().decode_prep_append(qkv, v, cos_all, sin_all, pos_flat, cache.k[i], cache.v[i],
@@ -342,8 +421,15 @@ class InferenceEngine:
                 q, k = ops.qk_prep_fwd(q4, k4, cos, sin)
             v4 = _heads(v, B, T, KV, D)
             table = cache.table(i)
-            ops.kv_append(cache.k[i], cache.v[i], table, pos_win if cache.is_windowed[i] else pos, k, v4)
-            if decode:
+            if mx:
+                cache.append(i, pos, k, v4)
+                attn = ops.paged_decode_attention_mx(q[:, 0], cache.k[i], cache.v[i], cache.k_scale[i], cache.v_scale[i],
+                                                     table, new_lens, wl).view(B, 1, H, D)
+            else:
+                ops.kv_append(cache.k[i], cache.v[i], table, pos_win if cache.is_windowed[i] else pos, k, v4)
+            if mx:
+                pass
+            elif decode:
                 attn = ops.paged_decode_attention(q[:, 0], cache.k[i], cache.v[i], table,
                                                   new_lens, wl).view(B, 1, H, D)
             elif t0 == 0:
@@ -368,6 +454,70 @@ class InferenceEngine:
         xn, _ = ops.rmsnorm_fwd(x_pre)
         return xn
 
+    @torch.no_grad()
+    def _forward_chunk(self, cache: PagedKVCache, tokens: torch.Tensor, counts: List[int]) -> torch.Tensor:
+        """The first counts[b] of tokens [B, T] are appended to sequence b, wherever it stands; the rest of the row is
+        padding. Every new token attends over the pages, so what a token sees does not depend on how its sequence
+        was cut into chunks. Returns the final normalised hidden states [B, T, C] (rows of padding are arbitrary)."""
+        cfg, m, P = self.cfg, self.model, self.model.params
+        B, T = tokens.shape
+        H, KV, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+        M, dev = B * T, self.device
+        cache.prepare_chunk(counts)
+        n_new = torch.tensor(counts, dtype=torch.int32, device=dev)
+        t = torch.arange(T, dtype=torch.int32, device=dev)[None]
+        real = t < n_new[:, None]
+        tok = torch.where(real, tokens.to(torch.int32), torch.zeros_like(tokens, dtype=torch.int32)).reshape(-1)
+        emb, _ = ops.rmsnorm_fwd(ops.embedding_fwd(tok, P.v("transformer.wte.weight")))
+        prev = torch.where((cache.seq_lens > 0)[:, None], cache.prev_emb, torch.zeros_like(cache.prev_emb))
+        x0, _ = ops.smear_fwd(emb, P.v("smear_gate.weight"), m._lam("smear_lambda"), T, prev=prev)
+        at = (n_new.long() - 1).clamp_min(0)
+        last = emb.view(B, T, -1)[torch.arange(B, device=dev), at]
+        cache.prev_emb.copy_(torch.where((n_new > 0)[:, None], last, cache.prev_emb))
+        pos = cache.seq_lens[:, None] + t
+        rope_pos = torch.where(real, pos, torch.zeros_like(pos)).contiguous()
+        pos = torch.where(real, pos, torch.full_like(pos, -1)).contiguous()
+        new_lens = cache.seq_lens + n_new
+        cos_all, sin_all = self._rope(cache.max_seq)
+        kernels = dev.type == "cuda" and ops.get_mode() == "kernels"
+        if not kernels:
+            cos, sin = cos_all[rope_pos.long()], sin_all[rope_pos.long()]
+        x = x0
+        x_backout = None
+        for i in range(cfg.num_layers):
+            xr, h, _ = ops.blend_norm_fwd(x, x0, m._lam("resid_lambdas", i), m._lam("x0_lambdas", i))
+            wqkv = P.qkv_view(i)
+            if wqkv is not None:
+                qkv = ops.linear_fwd(h, wqkv)
+                q_pre, k_pre = qkv[:, : cfg.query_dim], qkv[:, cfg.query_dim: cfg.query_dim + cfg.kv_dim]
+                v = qkv[:, cfg.query_dim + cfg.kv_dim:]
+            else:
+                q_pre, k_pre, v = (ops.linear_fwd(h, m._w(i, f"attn.c_{n}")) for n in "qkv")
+            if cfg.has_value_embedding(i):
+                ve = ops.embedding_fwd(tok, P.v(f"value_embeds.{i}.weight"))
+                v, _ = ops.value_gate_fwd(h, ve, m._w(i, "attn.ve_gate"), v, D)
+            q4, k4, v4 = _heads(q_pre, B, T, H, D), _heads(k_pre, B, T, KV, D), _heads(v, B, T, KV, D)
+            if kernels:
+                q, k = ops.cuda_module().qk_prep_fwd(q4, k4, cos_all, sin_all, positions=rope_pos.view(-1))
+            else:
+                q, k = ops.qk_prep_fwd(q4, k4, cos, sin)
+            cache.append(i, pos, k, v4)
+            ks, vs = (None, None) if cache.k_scale is None else (cache.k_scale[i], cache.v_scale[i])
+            attn = ops.paged_chunk_attention(q, cache.k[i], cache.v[i], cache.table(i), new_lens, n_new,
+                                             cfg.window_left(i), k_scale=ks, v_scale=vs)
+            x_mid = ops.linear_fwd(attn.reshape(M, H * D), m._w(i, "attn.c_proj"), residual=xr)
+            h2, _ = ops.rmsnorm_fwd(x_mid)
+            act = ops.linear_relu2_act_fwd(h2, m._w(i, "mlp.c_fc"))
+            x = ops.linear_fwd(act, m._w(i, "mlp.c_proj"), residual=x_mid)
+            if i == cfg.backout_layer:
+                x_backout = x
+        cache.seq_lens.add_(n_new)
+        for b, n in enumerate(counts):
+            cache.lens_host[b] += n
+        cache.has_prev = True
+        xn, _ = ops.rmsnorm_fwd(ops.backout_fwd(x, x_backout, m._lam("backout_lambda")))
+        return xn.view(B, T, -1)
+
     def _greedy(self, xn_rows: torch.Tensor) -> torch.Tensor:
         """Token ids of the largest logit per row (int64). The soft cap is monotonic, so on the kernel path the
         arg-max is taken over the bf16 logits directly and the fp32 capped copy is never made."""
@@ -391,6 +541,8 @@ class InferenceEngine:
         B, T = tokens.shape
         if max(cache.lens_host) + T > cache.max_seq:
             raise ValueError("prompt does not fit the KV cache")
+        if cache.k_scale is not None:
+            return self.extend(cache, tokens)
         xn = self._forward(cache, tokens, decode=False)
         return self._logits(xn.view(B, T, -1)[:, -1])
 
@@ -400,10 +552,14 @@ class InferenceEngine:
         together (one pass per distinct length). Returns the logits of every prompt's last position [B, vocab]."""
         if len(prompts) != cache.batch:
             raise ValueError("one prompt per sequence of the cache")
+        if any(len(p) == 0 for p in prompts):
+            raise ValueError("empty prompt")
+        if cache.k_scale is not None:
+            longest = max(len(p) for p in prompts)
+            tok = torch.tensor([list(p) + [0] * (longest - len(p)) for p in prompts], dtype=torch.long, device=self.device)
+            return self.extend(cache, tok, [len(p) for p in prompts])
         groups = {}
         for r, p in enumerate(prompts):
-            if len(p) == 0:
-                raise ValueError("empty prompt")
             groups.setdefault(len(p), []).append(r)
         out = None
         for length, rows in sorted(groups.items()):
@@ -416,6 +572,43 @@ class InferenceEngine:
                 out = torch.empty(cache.batch, lg.shape[1], dtype=lg.dtype, device=lg.device)
             out[torch.as_tensor(rows, device=lg.device)] = lg
         cache.has_prev = True
+        return out
+
+    @torch.no_grad()
+    def extend(self, cache: PagedKVCache, tokens: torch.Tensor, counts: Optional[Sequence[int]] = None,
+               all_logits: bool = False) -> torch.Tensor:
+        """Append the first counts[b] (default: all) of tokens [B, T] to sequence b, each sequence at its own position:
+        prompts of different lengths, a further turn of a conversation, drafted tokens to verify. Returns the logits of
+        every sequence's last new token [B, vocab] (zeros where counts[b] is 0) or, with `all_logits`, those of all new
+        tokens [B, T, vocab] (zeros behind counts[b]). Longer inputs than the cache's windowed layers hold at once
+        go through in pieces."""
+        if tokens.dim() != 2 or tokens.shape[0] != cache.batch:
+            raise ValueError("extend: tokens must be [sequences of the cache, T]")
+        tokens = tokens.to(self.device)
+        B, T = tokens.shape
+        counts = [T] * B if counts is None else [int(n) for n in counts]
+        if len(counts) != B or any(n < 0 or n > T for n in counts):
+            raise ValueError("extend: counts must hold one number in [0, T] per sequence")
+        if any(have + n > cache.max_seq for have, n in zip(cache.lens_host, counts)):
+            raise ValueError("sequence does not fit the KV cache")
+        V = self.cfg.vocab_size
+        out = torch.zeros((B, T, V) if all_logits else (B, V), dtype=torch.float32, device=self.device)
+        for start in range(0, max(counts, default=0), cache.chunk):
+            piece = tokens[:, start:start + cache.chunk]
+            n = [min(max(c - start, 0), piece.shape[1]) for c in counts]
+            xn = self._forward_chunk(cache, piece, n)
+            if all_logits:
+                rows = [(b, i) for b in range(B) for i in range(n[b])]
+            else:
+                rows = [(b, c - start - 1) for b, c in enumerate(counts) if start < c <= start + cache.chunk]
+            if not rows:
+                continue
+            b, i = (torch.tensor(x, device=self.device) for x in zip(*rows))
+            lg = self._logits(xn[b, i]).to(out.dtype)
+            if all_logits:
+                out[b, i + start] = lg
+            else:
+                out[b] = lg
         return out
 
     @torch.no_grad()
@@ -523,6 +716,11 @@ class GenerateParams:
     stop_id: int = -1
     bos_id: int = -1
     stop_ids: Sequence[int] = ()
+    # Nucleus and min-p sampling (see ops.sample_rows) run on the device, from the same per-row streams of random
+    # numbers; `device_sampling` takes that path for temperature and top-k alone too, where the default draws on the host.
+    top_p: float = 1.0
+    min_p: float = 0.0
+    device_sampling: bool = False
 
 
 @dataclass
@@ -565,8 +763,16 @@ def generate_multi(engine: InferenceEngine, prompts, params: GenerateParams,
     # greedy decoding without forced tokens never needs the logits after the prefill: the step returns token ids
     greedy_ids = (not params.temperature > 0.0) and forced is None
     pred = None
+    on_device = params.temperature > 0.0 and (params.top_p < 1.0 or params.min_p > 0.0 or params.device_sampling)
+    if on_device:
+        from ..data import native
+        uniforms = torch.from_numpy(native.sample_uniforms(params.seed, range(rows), 0, params.max_tokens)).to(dev)
     for step in range(params.max_tokens):
-        nxt = pred if pred is not None else sample(logits, params.temperature, params.top_k, params.seed, row_ids, step)
+        if on_device:
+            nxt = ops.sample_rows(logits, uniforms[step], params.temperature, params.top_k, params.top_p, params.min_p)
+        else:
+            nxt = (pred if pred is not None else
+                   sample(logits, params.temperature, params.top_k, params.seed, row_ids, step))
         was_forced = [False] * rows
         if forced is not None:
             host = nxt.tolist()

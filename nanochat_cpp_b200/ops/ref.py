@@ -749,10 +749,10 @@ def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, 
     """Attention of a chunk of new tokens over the paged cache, their own keys included (append first). q [B, T, H, D];
     the first q_lens[b] (None: T) rows of sequence b are its last q_lens[b] positions of seq_lens[b]. Row t sees keys
     j <= its position p = seq_lens[b] - q_lens[b] + t with p - j <= window_left. With `k_scale` / `v_scale` the pools
-    are MXFP8 (see `kv_append_mx`), without them they have the type of q. Rows at or behind q_lens[b] and rows that
+    are MXFP8 (see `kv_append_mx`), without them they have the type of q. The kernels take D = 64 or 128. Rows at or behind q_lens[b] and rows that
     see no key are zero. A key past the page table or on a page outside the pool is left out."""
     name = "paged_chunk_attention"
-    _check(q.dim() == 4 and q.stride(3) == 1 and q.shape[3] in (64, 128), f"{name}: q must be [B, T, H, D], D 64 or 128")
+    _check(q.dim() == 4 and q.stride(3) == 1, f"{name}: q must be [B, T, H, D] with dense channels")
     B, T, H, D = q.shape
     _check((k_scale is None) == (v_scale is None), f"{name}: give both scales or neither")
     if k_scale is not None:
