@@ -9,13 +9,14 @@
 // memory in a matrix layout. tcgen05 would need 128-row operands staged by another copy; there is nothing to win at 8.
 // The fragment layouts leave the order of the contraction index and of the output channels free, so a lane owns
 // contiguous channels: D/4 of a key row for S^T = K Q^T (one MX block for D = 128), D/8 of four value rows for
-// O^T = V^T P^T. Each lane copies its own bytes with cp.async into a ring private to its warp and reads back only those:
-// no CTA barrier in the main loop. P^T moves from the accumulator to the operand layout by two 8x8 transposes.
+// O^T = V^T P^T. Rows arrive by cp.async, whole rows per instruction (lanes that took their own quarter row asked L2
+// for every 32-byte sector twice), in a ring private to the warp: no CTA barrier in the main loop. P^T moves from the accumulator to the operand layout by two 8x8 transposes.
 //
-// grid (key splits, kv heads x row blocks, sequences). Warps of a CTA take 16-key tiles in turn; their partial
-// results meet in shared memory, those of different splits in a combine kernel. The reference maximum of a row is raised only
-// when a score exceeds it by 2^8 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
-// Probabilities are rounded to bf16 for the second product; the sum is taken of the rounded values, in fp32.
+// A warp is a unit of its own: it takes one run of keys (`split_keys`) of one sequence, kv head and block of rows, and
+// writes its partial sums; a combine kernel joins the runs of a row. Nothing in the CTA waits for anything else, and
+// sequences of different lengths even out over many equal units. The reference maximum of a row is raised only when a
+// score exceeds it by 2^8 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
+// Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -36,6 +37,7 @@ namespace {
 
 constexpr int kTile = 16;        // keys per warp step
 constexpr int kStages = 3;       // ring depth per warp
+constexpr int kMaxRun = 512;     // keys of one warp's run at most: its page numbers fit one per lane
 constexpr float kRaise = 8.0f;   // log2 units
 constexpr float kNoMax = -1.0e30f;
 
@@ -44,12 +46,43 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+template <bool F16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two E4M3 codes (the low or the high half of w) as f16: exact
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, hi;\n}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float pow2(int d) { return __uint_as_float(static_cast<uint32_t>(min(max(127 + d, 0), 255)) << 23); }
+// 2^d for d <= 0 (0 below the range of fp32)
+__device__ __forceinline__ float pow2_neg(int d) { return __uint_as_float(static_cast<uint32_t>(max(127 + d, 0)) << 23); }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -95,45 +128,47 @@ __device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int b, int r0,
 
 template <int D, bool MX>
 struct Ring {
-  static constexpr int kB = MX ? 1 : 2;                       // bytes per element
-  static constexpr int kK = D / 4 * kB, kV = D / 8 * kB;      // bytes a lane owns of one key / value row
+  static constexpr int kRow = D * (MX ? 1 : 2);               // bytes of a key or value row
+  static constexpr int kLanes = kRow / 16;                    // lanes that copy one row
+  static constexpr int kCopies = 16 * kLanes / 32;            // copies per lane and side
   static constexpr int kScale = 16 * (D / 32);                // scale bytes of a tile, one side
-  static constexpr int kOffV = 32 * 2 * kK;
-  static constexpr int kOffS = kOffV + 32 * 4 * kV;
-  static constexpr int kOffPage = kOffS + (MX ? 2 * kScale : 0);
-  static constexpr int kStage = (kOffPage + 16 + 15) / 16 * 16;
-  static constexpr int kWarps = MX ? 8 : 4;                   // about 100 KB of ring either way: two CTAs per SM
-  static constexpr int kBytes = kWarps * kStages * kStage;
-};
-
-template <int D, bool MX, int NT>
-struct RowsSmem {
-  using R = Ring<D, MX>;
-  static constexpr int kRows = 8 * NT;
-  static constexpr int kTree = R::kWarps / 2 * (D / 16 * NT * 4) * 32 * 4;   // partial sums of half of the warps
-  static constexpr int kMain = R::kBytes > kTree ? R::kBytes : kTree;
-  static constexpr int kOffML = kMain;
-  static constexpr int kTotal = kMain + R::kWarps * kRows * 2 * 4;
+  static constexpr int kOffV = 16 * kRow;
+  static constexpr int kOffS = 2 * kOffV;
+  static constexpr int kOffPage = kOffS + (MX ? 2 * kScale : 0);   // which keys are usable, where a tile spans pages
+  static constexpr int kStage = kOffPage + 16;
+  static constexpr int kBytes = kStages * kStage;
+  // Place of 16-byte piece `p` of row `key` inside the row, chosen so that the eight lanes of a 16-byte read phase hit
+  // different banks: they read pieces of keys (0, 1) at distance kRow / 64 on the key side, and pieces (0, 1) times
+  // kRow / 128 of keys 0, 2, 4, 6 on the value side.
+  static __device__ __forceinline__ int place_k(int key, int p) {
+    if constexpr (kRow == 256) return p ^ ((p >> 3) + 2 * (key & 1));
+    else if constexpr (kRow == 128) return p ^ (key & 1);
+    else return p;
+  }
+  static __device__ __forceinline__ int place_v(int key, int p) {
+    if constexpr (kRow == 256) return p ^ (4 * ((key >> 1) & 1) + ((key >> 2) & 1));
+    else if constexpr (kRow == 128) return p ^ (2 * ((key >> 1) & 3));
+    else return p ^ ((key >> 1) & 3);
+  }
 };
 
 // P16: page_size is a multiple of 16, so a tile lies in one page.
 template <int D, bool MX, int NT, bool P16>
-__global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) paged_rows_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(const PagedAttnArgs a) {
   using R = Ring<D, MX>;
-  using L = RowsSmem<D, MX, NT>;
-  constexpr int W = R::kWarps, ROWS = L::kRows;
+  constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
   NC_PDL_PROLOGUE();
   const int G = a.H / a.KV;
+  const int lane = threadIdx.x, g8 = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.KV, rb = blockIdx.y / a.KV, b = blockIdx.z;
   const int r0 = rb * ROWS, row_count = min(ROWS, a.T * G - r0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, c = lane & 3;
   const Range rg = range_of(a, b, r0, ROWS);
   const int split_tiles = a.split_keys / kTile;
   const int t0 = rg.tile0 + split * split_tiles;
-  const int my_tiles = min(rg.tiles - split * split_tiles, split_tiles);
-  if (split > 0 && my_tiles <= 0) return;
-  if (split == 0 && threadIdx.x == 0 && rg.pmax >= static_cast<long long>(a.max_pages) * a.page_size && a.status != nullptr)
+  const int count = min(rg.tiles - split * split_tiles, split_tiles);
+  if (split > 0 && count <= 0) return;
+  if (split == 0 && lane == 0 && rg.pmax >= static_cast<long long>(a.max_pages) * a.page_size && a.status != nullptr)
     atomicCAS(a.status, 0, kErrBadIndex);   // keys past the page table are left out
   const float sl = a.scale * 1.4426950408889634f;
 
@@ -141,8 +176,11 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
     const int t = (r0 + r) / G, h = kvh * G + (r0 + r) % G;
     return a.q + b * a.q_stride_b + t * a.q_stride_t + h * a.q_stride_h;
   };
-  // Q as the B operand: row nt * 8 + g8, contraction step s covers channels c * D/4 + 4 s .. + 3
+  // Q as the B operand: row nt * 8 + g8, contraction step s covers channels c * D/4 + 4 s .. + 3. For MXFP8 the products
+  // run in f16, which holds E4M3 codes exactly; a row of Q is brought below 2^15 by a power of two, so that bf16's
+  // 8 bits survive down to 2^-29 of the row's largest magnitude, and the power goes into the row's score factor.
   uint32_t qf[NT][D / 8];
+  float row_factor[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g8;
@@ -153,8 +191,30 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
       const uint4 x = ok ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0, 0, 0, 0);
       qf[nt][4 * i] = x.x, qf[nt][4 * i + 1] = x.y, qf[nt][4 * i + 2] = x.z, qf[nt][4 * i + 3] = x.w;
     }
+    row_factor[nt] = sl;
+    if constexpr (MX) {
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) mx = __vmaxu2(mx, qf[nt][i] & 0x7fff7fffu);
+      mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const uint32_t top = max(mx & 0xffffu, mx >> 16);
+      int e = static_cast<int>(top >> 7);                  // biased exponent of the largest magnitude
+      if (top == 0 || top >= 0x7f80) e = 127 + 14;         // nothing to scale: zeros, infinities, NaN
+      e = max(e, 15);
+      const float up = __uint_as_float(static_cast<uint32_t>(min(127 + 14 + 127 - e, 254)) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(max(e - 14, 1)) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) qf[nt][i] = pack_f16(bf16_lo(qf[nt][i]) * up, bf16_hi(qf[nt][i]) * up);
+      row_factor[nt] = down * sl;
+    }
   }
-  int pos[NT][2];   // positions of the rows this lane holds scores of (accumulator columns 2c, 2c + 1)
+  float factor[NT][2];   // score factor of the rows this lane holds scores of (accumulator columns 2c, 2c + 1)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) factor[nt][e] = __shfl_sync(0xffffffffu, row_factor[nt], (2 * c + e) * 4);
+  int pos[NT][2];        // and their positions
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -172,18 +232,56 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][nt][e] = 0.0f;
-  float m[NT][2], l[NT][2];
+  float m[NT][2];        // reference maximum, in units of the exponent
+  float l[NT][4];        // sums of the rounded probabilities: P^T times a row of ones on the tensor core
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = kNoMax, l[nt][0] = l[nt][1] = 0.0f;
+  for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = kNoMax, l[nt][0] = l[nt][1] = l[nt][2] = l[nt][3] = 0.0f;
+  // MXFP8: codes enter the products as code * 2^(b - ref), ref the largest scale byte of the run so far (one for keys, one
+  // for values): f16 holds that exactly as long as scales differ by no more than 2^15, and to 2^-33 of the largest
+  // beyond. The scores take 2^(k_ref - 127) into their factor; a larger v_ref scales down what has been summed.
+  int k_ref = 0, v_ref = 0;
+  float k_unit = 0.0f;
 
-  uint8_t* ring = smem + warp * (kStages * R::kStage);
-  const int count = my_tiles > warp ? (my_tiles - warp + W - 1) / W : 0;
+  uint8_t* ring = smem;
   const int* table = a.page_table + static_cast<long long>(b) * a.max_pages;
-  const long long key_stride = static_cast<long long>(a.KV) * D * R::kB;   // bytes
-  const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + static_cast<long long>(kvh) * D * R::kB;
-  const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + static_cast<long long>(kvh) * D * R::kB;
+  const uint32_t stride = static_cast<uint32_t>(a.KV) * R::kRow;   // bytes from a token to the next
+  // what this lane copies: piece lane % kLanes of rows lane / kLanes, and every 32 / kLanes-th after it
+  const int row_l = lane / R::kLanes, piece = lane % R::kLanes;
+  constexpr int kStep = 32 / R::kLanes;
+  const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + kvh * R::kRow + piece * 16;
+  const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + kvh * R::kRow + piece * 16;
+  // and reads: its quarter of key row g8, its eighth of value row 2c
+  int k_at[R::kRow / 64], v_at[R::kRow >= 128 ? R::kRow / 128 : 1];
+#pragma unroll
+  for (int x = 0; x < R::kRow / 64; ++x) k_at[x] = g8 * R::kRow + R::place_k(g8, c * (R::kRow / 64) + x) * 16;
+  if constexpr (R::kRow >= 128) {
+#pragma unroll
+    for (int x = 0; x < R::kRow / 128; ++x) v_at[x] = R::kOffV + 2 * c * R::kRow + R::place_v(2 * c, g8 * (R::kRow / 128) + x) * 16;
+  } else {
+    v_at[0] = R::kOffV + 2 * c * R::kRow + R::place_v(2 * c, g8 / 2) * 16 + (g8 & 1) * 8;
+  }
+  // P16: lane i holds the i-th page of the run, and `at_page`, `in_page` follow the tiles that are requested
   const int tiles_per_page = P16 ? a.page_size / kTile : 1;
-  int page_ids = -1;   // P16: lane i holds the page of this warp's tile 32 * (block of tiles) + i
+  int page_ids = -1, at_page = 0, in_page = 0;
+  unsigned bad_tiles = 0;   // P16: bit i: the page of tile i is unmapped or outside the pool
+  if constexpr (P16) {
+    const int first = t0 / tiles_per_page;
+    in_page = t0 - first * tiles_per_page;
+    if (count > 0 && first + lane <= (t0 + count - 1) / tiles_per_page) page_ids = table[first + lane];
+    const int mine = __shfl_sync(0xffffffffu, page_ids, (in_page + lane) / tiles_per_page);
+    bad_tiles = __ballot_sync(0xffffffffu, lane < count && (mine < 0 || mine >= a.num_pages));
+    if (bad_tiles != 0 && lane == 0 && a.status != nullptr) atomicCAS(a.status, 0, kErrBadIndex);
+  }
+  const uint8_t* s_lane = nullptr;
+  uint32_t s_dst = 0, s_stride = 0;
+  constexpr int kScaleLanes = MX ? R::kScale / 16 : 1;   // 16-byte pieces of a tile's scales, one side
+  if constexpr (MX) {
+    const int part = lane % kScaleLanes;
+    const bool is_v = lane >= kScaleLanes;
+    s_lane = (is_v ? a.v_scale : a.k_scale) + static_cast<long long>(kvh) * a.page_size * (D / 32) + part * 16;
+    s_dst = R::kOffS + (is_v ? R::kScale : 0) + part * 16;
+    s_stride = static_cast<uint32_t>(a.KV * a.page_size * (D / 32));
+  }
 
   // row (page * page_size + slot) of a key, -1: not in the cache
   auto key_row = [&](int key) -> long long {
@@ -191,75 +289,44 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
     const int page = table[key / a.page_size];
     return page >= 0 && page < a.num_pages ? static_cast<long long>(page) * a.page_size + key % a.page_size : -1;
   };
+  int put = 0, get = 0;   // stages that are written and read next
   auto issue = [&](int i) {
-    uint8_t* st = ring + (i % kStages) * R::kStage;
+    uint8_t* st = ring + put * R::kStage;
+    put = put + 1 == kStages ? 0 : put + 1;
     const uint32_t dst = smem_u32(st);
-    const int tile = t0 + warp + W * i;
-    const int key0 = tile * kTile;
+    const int key0 = (t0 + i) * kTile;
     if constexpr (P16) {
-      if ((i & 31) == 0) {
-        const int mine = t0 + warp + W * (i + lane);
-        page_ids = i + lane < count ? table[mine / tiles_per_page] : -1;
-      }
-      const int page = __shfl_sync(0xffffffffu, page_ids, i & 31);
-      const bool page_ok = page >= 0 && page < a.num_pages;
-      if (!page_ok && lane == 0 && a.status != nullptr) atomicCAS(a.status, 0, kErrBadIndex);
-      const long long row0 = page_ok ? static_cast<long long>(page) * a.page_size + (tile % tiles_per_page) * kTile : 0;
+      // a page that is none of the pool's stands for page 0: its rows are requested as zeros
+      const bool page_ok = ((bad_tiles >> i) & 1) == 0;
+      const int id = __shfl_sync(0xffffffffu, page_ids, at_page);
+      const uint32_t page = page_ok ? id : 0, slot0 = in_page * kTile;
+      if (++in_page == tiles_per_page) in_page = 0, ++at_page;
+      // all 16 rows lie inside the page, wanted or not
+      const unsigned long long base = (static_cast<unsigned long long>(page) * a.page_size + slot0 + row_l) * stride;
+      const uint8_t *ks = kp + base, *vs = vp + base;
+      auto rows_in = [&](auto wanted) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int key = g8 + 8 * hh;
-        const bool ok = page_ok && key0 + key >= rg.lo && key0 + key < rg.hi;
-        const uint8_t* src = kp + (row0 + key) * key_stride + c * R::kK;
-#pragma unroll
-        for (int x = 0; x < R::kK / 16; ++x)
-          copy_async<16>(dst + ((hh * (R::kK / 16) + x) * 32 + lane) * 16, ok ? src + 16 * x : static_cast<const uint8_t*>(a.k_pool), ok);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = 2 * c + (j & 1) + 8 * (j >> 1);
-        const bool ok = page_ok && key0 + key >= rg.lo && key0 + key < rg.hi;
-        const uint8_t* src = vp + (row0 + key) * key_stride + g8 * R::kV;
-        if constexpr (R::kV == 8)
-          copy_async<8>(dst + R::kOffV + (j * 32 + lane) * 8, ok ? src : static_cast<const uint8_t*>(a.v_pool), ok);
-        else
-#pragma unroll
-          for (int x = 0; x < R::kV / 16; ++x)
-            copy_async<16>(dst + R::kOffV + ((j * (R::kV / 16) + x) * 32 + lane) * 16,
-                           ok ? src + 16 * x : static_cast<const uint8_t*>(a.v_pool), ok);
-      }
-      if constexpr (MX) {   // 16 tokens x D/32 scale bytes of one page and head are contiguous
-        constexpr int kLanes = R::kScale / 16;
-        if (lane < 2 * kLanes) {
-          const bool is_v = lane >= kLanes;
-          const int part = is_v ? lane - kLanes : lane;
-          const uint8_t* base = is_v ? a.v_scale : a.k_scale;
-          const long long off = page_ok ? ((static_cast<long long>(page) * a.KV + kvh) * a.page_size +
-                                           (tile % tiles_per_page) * kTile) * (D / 32) + part * 16 : 0;
-          copy_async<16>(dst + R::kOffS + (is_v ? R::kScale : 0) + part * 16, base + off, page_ok);
+        for (int x = 0; x < R::kCopies; ++x) {
+          const int key = row_l + x * kStep;
+          const bool ok = wanted(key);
+          copy_async<16>(dst + key * R::kRow + R::place_k(key, piece) * 16, ks + x * kStep * stride, ok);
+          copy_async<16>(dst + R::kOffV + key * R::kRow + R::place_v(key, piece) * 16, vs + x * kStep * stride, ok);
         }
+      };
+      if (page_ok && key0 >= rg.lo && key0 + kTile <= rg.hi) rows_in([](int) { return true; });
+      else rows_in([&](int k) { return page_ok && key0 + k >= rg.lo && key0 + k < rg.hi; });
+      if constexpr (MX) {   // 16 tokens x D/32 scale bytes of one page and head are contiguous
+        if (lane < 2 * kScaleLanes)
+          copy_async<16>(dst + s_dst, s_lane + static_cast<unsigned long long>(page) * s_stride + slot0 * (D / 32), page_ok);
       }
-      if (lane == 0) *reinterpret_cast<int*>(st + R::kOffPage) = page_ok;
     } else {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const long long row = key_row(key0 + g8 + 8 * hh);
-        const uint8_t* src = kp + row * key_stride + c * R::kK;
-#pragma unroll
-        for (int x = 0; x < R::kK / 16; ++x)
-          copy_async<16>(dst + ((hh * (R::kK / 16) + x) * 32 + lane) * 16,
-                         row >= 0 ? src + 16 * x : static_cast<const uint8_t*>(a.k_pool), row >= 0);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const long long row = key_row(key0 + 2 * c + (j & 1) + 8 * (j >> 1));
-        const uint8_t* src = vp + row * key_stride + g8 * R::kV;
-        if constexpr (R::kV == 8)
-          copy_async<8>(dst + R::kOffV + (j * 32 + lane) * 8, row >= 0 ? src : static_cast<const uint8_t*>(a.v_pool), row >= 0);
-        else
-#pragma unroll
-          for (int x = 0; x < R::kV / 16; ++x)
-            copy_async<16>(dst + R::kOffV + ((j * (R::kV / 16) + x) * 32 + lane) * 16,
-                           row >= 0 ? src + 16 * x : static_cast<const uint8_t*>(a.v_pool), row >= 0);
+      for (int x = 0; x < R::kCopies; ++x) {
+        const int key = row_l + x * kStep;
+        const long long row = key_row(key0 + key);
+        const unsigned long long base = static_cast<unsigned long long>(row >= 0 ? row : 0) * stride;
+        copy_async<16>(dst + key * R::kRow + R::place_k(key, piece) * 16, kp + base, row >= 0);
+        copy_async<16>(dst + R::kOffV + key * R::kRow + R::place_v(key, piece) * 16, vp + base, row >= 0);
       }
       const int key = key0 + (lane & 15);
       const long long row = key_row(key);
@@ -288,58 +355,82 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
     __syncwarp();    // this stage has arrived for every lane; the stage before it has been read by every lane
     if (i + kStages - 1 < count) issue(i + kStages - 1);
     copy_commit();
-    const uint8_t* st = ring + (i % kStages) * R::kStage;
-    const int key0 = (t0 + warp + W * i) * kTile;
-    const int page_info = *reinterpret_cast<const int*>(st + R::kOffPage);
-    const bool edge = key0 < all_lo || key0 + kTile > all_hi || (P16 ? page_info == 0 : page_info != 0xffff);
+    const uint8_t* st = ring + get * R::kStage;
+    get = get + 1 == kStages ? 0 : get + 1;
+    const int key0 = (t0 + i) * kTile;
+    const int page_info = P16 ? 0 : *reinterpret_cast<const int*>(st + R::kOffPage);
+    const bool tile_ok = P16 ? ((bad_tiles >> i) & 1) == 0 : page_info == 0xffff;
+    const bool edge = key0 < all_lo || key0 + kTile > all_hi || !tile_ok;
     auto key_ok = [&](int k) {   // key0 + k holds a key of the cache that some row may see
-      return key0 + k >= rg.lo && key0 + k < rg.hi && (P16 ? page_info != 0 : ((page_info >> k) & 1) != 0);
+      return key0 + k >= rg.lo && key0 + k < rg.hi && (P16 ? tile_ok : ((page_info >> k) & 1) != 0);
     };
 
     // ---- S^T = K Q^T
     float s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-    uint32_t f1[2], f2[2];
-    bool far = false;
-    if constexpr (MX) {
+    float s2[NT][4];   // two chains of products, added at the end
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const uint32_t sb = st[R::kOffS + (g8 + 8 * hh) * (D / 32) + c * (D / 4) / 32];
-        f1[hh] = mx_factor_first(sb) * 0x10001u, f2[hh] = mx_factor_second(sb) * 0x10001u;
-        far = far || sb > 134u;
+    for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
+    uint32_t f1[2], g1[2];   // factors of this lane's share of keys g8, g8 + 8 and of value rows (2c, 2c + 1), (2c + 8, 2c + 9)
+    if constexpr (MX) {
+      const uint8_t* sk = st + R::kOffS + g8 * (D / 32) + c * (D / 4) / 32;
+      const uint8_t* sw = st + R::kOffS + R::kScale + 2 * c * (D / 32) + g8 * (D / 8) / 32;
+      int bk[2] = {sk[0], sk[8 * (D / 32)]};
+      int bv[4] = {sw[0], sw[D / 32], sw[8 * (D / 32)], sw[9 * (D / 32)]};
+      if (__any_sync(0xffffffffu, max(bk[0], bk[1]) > k_ref || max(max(bv[0], bv[1]), max(bv[2], bv[3])) > v_ref)) {
+        // rare: a larger scale than any so far. NaN (255: the codes are NaN already) and keys that are none count for nothing
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (bv[j] == 255 || !key_ok(2 * c + (j & 1) + 8 * (j >> 1))) bv[j] = 0;
+        k_ref = max(k_ref, __reduce_max_sync(0xffffffffu, max(bk[0], bk[1])));
+        k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
+        const int next = max(v_ref, __reduce_max_sync(0xffffffffu, max(max(bv[0], bv[1]), max(bv[2], bv[3]))));
+        const float alpha = pow2_neg(v_ref - next);
+        v_ref = next;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[d][nt][e] *= alpha;
       }
-      far = __any_sync(0xffffffffu, far);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float f = pow2_neg(bk[j] - k_ref);
+        f1[j] = pack_f16(f, f);
+        g1[j] = pack_f16(pow2_neg(bv[2 * j] - v_ref), pow2_neg(bv[2 * j + 1] - v_ref));
+      }
     }
 #pragma unroll
-    for (int x = 0; x < R::kK / 16; ++x) {
-      const uint4 w0 = *reinterpret_cast<const uint4*>(st + (x * 32 + lane) * 16);
-      const uint4 w1 = *reinterpret_cast<const uint4*>(st + ((R::kK / 16 + x) * 32 + lane) * 16);
+    for (int x = 0; x < R::kRow / 64; ++x) {
+      const uint4 w0 = *reinterpret_cast<const uint4*>(st + k_at[x]);
+      const uint4 w1 = *reinterpret_cast<const uint4*>(st + k_at[x] + 8 * R::kRow);
       const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
       if constexpr (MX) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          uint32_t fa[4];
-          mx_spread(u0[y], fa[0], fa[2]);
-          mx_spread(u1[y], fa[1], fa[3]);
+          const uint32_t fa[4] = {mul_f16x2(codes_lo(u0[y]), f1[0]), mul_f16x2(codes_lo(u1[y]), f1[1]),
+                                  mul_f16x2(codes_hi(u0[y]), f1[0]), mul_f16x2(codes_hi(u1[y]), f1[1])};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) fa[e] = mul_bf16x2(fa[e], f1[e & 1]);
-          if (far) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) fa[e] = mul_bf16x2(fa[e], f2[e & 1]);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<true>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
         }
       } else {
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const uint32_t fa[4] = {u0[2 * y], u1[2 * y], u0[2 * y + 1], u1[2 * y + 1]};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(s[nt], fa, qf[nt][2 * (2 * x + y)], qf[nt][2 * (2 * x + y) + 1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (2 * x + y)], qf[nt][2 * (2 * x + y) + 1]);
         }
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (MX ? factor[nt][e & 1] * k_unit : factor[nt][e & 1]);
 
     // ---- masks, running maximum, probabilities
     if (edge) {
@@ -355,7 +446,7 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) raise = raise || (s[nt][e] - m[nt][e & 1]) * sl > kRaise;
+      for (int e = 0; e < 4; ++e) raise = raise || s[nt][e] - m[nt][e & 1] > kRaise;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -364,9 +455,9 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
           float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][e + 2]));
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float alpha = fast_exp2((m[nt][e] - mx) * sl);
+          const float alpha = fast_exp2(m[nt][e] - mx);
           m[nt][e] = mx;
-          l[nt][e] *= alpha;
+          l[nt][e] *= alpha, l[nt][e + 2] *= alpha;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) acc[d][nt][e] *= alpha, acc[d][nt][e + 2] *= alpha;
         }
@@ -374,41 +465,28 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
     uint32_t pf[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float c0 = m[nt][0] * sl, c1 = m[nt][1] * sl;
-      const uint32_t p0 = pack_bf16(fast_exp2(s[nt][0] * sl - c0), fast_exp2(s[nt][1] * sl - c1));
-      const uint32_t p1 = pack_bf16(fast_exp2(s[nt][2] * sl - c0), fast_exp2(s[nt][3] * sl - c1));
-      l[nt][0] += bf16_lo(p0) + bf16_lo(p1);
-      l[nt][1] += bf16_hi(p0) + bf16_hi(p1);
-      pf[nt][0] = transpose_8x8(p0), pf[nt][1] = transpose_8x8(p1);
+      // f16 probabilities are taken 2^7 times too large (below 2^15): small ones keep their bits; the sums carry the factor too
+      const float c0 = m[nt][0] - (MX ? 7.0f : 0.0f), c1 = m[nt][1] - (MX ? 7.0f : 0.0f);
+      const float p0 = fast_exp2(s[nt][0] - c0), p1 = fast_exp2(s[nt][1] - c1);
+      const float p2 = fast_exp2(s[nt][2] - c0), p3 = fast_exp2(s[nt][3] - c1);
+      pf[nt][0] = transpose_8x8(MX ? pack_f16(p0, p1) : pack_bf16(p0, p1));
+      pf[nt][1] = transpose_8x8(MX ? pack_f16(p2, p3) : pack_bf16(p2, p3));
+      constexpr uint32_t kOne = MX ? 0x3c003c00u : 0x3f803f80u;
+      const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+      mma_16816<MX>(l[nt], ones, pf[nt][0], pf[nt][1]);
     }
 
     // ---- O^T += V^T P^T: keys 2c, 2c + 1 (low, high half of a register) and 2c + 8, 2c + 9
-    const uint8_t* sv = st + R::kOffV;
     if constexpr (MX) {
-      uint32_t g1[2], g2[2];
-      bool vfar = false;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint8_t* ss = st + R::kOffS + R::kScale + (2 * c + 8 * j) * (D / 32) + g8 * (D / 8) / 32;
-        uint32_t sa = ss[0], sb = ss[D / 32];
-        vfar = vfar || sa > 134u || sb > 134u;
-        g1[j] = mx_factor_first(sa) | (mx_factor_first(sb) << 16);
-        g2[j] = mx_factor_second(sa) | (mx_factor_second(sb) << 16);
-        if (edge) {   // a key outside the cache has codes of zero: its factor must be a number too
-          if (!key_ok(2 * c + 8 * j)) g1[j] &= 0xffff0000u, g2[j] &= 0xffff0000u;
-          if (!key_ok(2 * c + 8 * j + 1)) g1[j] &= 0xffffu, g2[j] &= 0xffffu;
-        }
-      }
-      vfar = __any_sync(0xffffffffu, vfar);
-      constexpr int kWords = R::kV / 4;
+      constexpr int kWords = R::kRow / 32;
       uint32_t v[4][kWords];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (kWords == 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sv + (j * 32 + lane) * 16);
+          const uint4 w = *reinterpret_cast<const uint4*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
           v[j][0] = w.x, v[j][1] = w.y, v[j][2] = w.z, v[j][3] = w.w;
         } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(sv + (j * 32 + lane) * 8);
+          const uint2 w = *reinterpret_cast<const uint2*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
           v[j][0] = w.x, v[j][1] = w.y;
         }
       }
@@ -417,116 +495,60 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
         uint32_t f[2][4];   // [key pair][channel 4y + .], each (first key, second key)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          mx_spread(__byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x5140), f[j][0], f[j][1]);
-          mx_spread(__byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x7362), f[j][2], f[j][3]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) f[j][e] = mul_bf16x2(f[j][e], g1[j]);
-          if (vfar) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[j][e] = mul_bf16x2(f[j][e], g2[j]);
-          }
+          const uint32_t ab = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x5140), cd = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x7362);
+          f[j][0] = mul_f16x2(codes_lo(ab), g1[j]), f[j][1] = mul_f16x2(codes_hi(ab), g1[j]);
+          f[j][2] = mul_f16x2(codes_lo(cd), g1[j]), f[j][3] = mul_f16x2(codes_hi(cd), g1[j]);
         }
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const uint32_t fa[4] = {f[0][2 * z], f[0][2 * z + 1], f[1][2 * z], f[1][2 * z + 1]};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<true>(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
         }
       }
     } else {
 #pragma unroll
-      for (int x = 0; x < R::kV / 16; ++x) {
+      for (int x = 0; x < R::kRow / 128; ++x) {
         uint4 w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(sv + ((j * (R::kV / 16) + x) * 32 + lane) * 16);
+        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(st + v_at[x] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const uint32_t v0 = (&w[0].x)[y], v1 = (&w[1].x)[y], v2 = (&w[2].x)[y], v3 = (&w[3].x)[y];
           const uint32_t fa[4] = {__byte_perm(v0, v1, 0x5410), __byte_perm(v0, v1, 0x7632), __byte_perm(v2, v3, 0x5410),
                                   __byte_perm(v2, v3, 0x7632)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816(acc[4 * x + y][nt], fa, pf[nt][0], pf[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(acc[4 * x + y][nt], fa, pf[nt][0], pf[nt][1]);
         }
       }
     }
   }
   copy_wait<0>();
-  __syncthreads();   // the ring is free: it becomes the exchange buffer of the warps
 
-  // ---- the warps' results meet
-  float* sm_m = reinterpret_cast<float*>(smem + L::kOffML);
-  float* sm_l = sm_m + W * ROWS;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
-      if (g8 == 0) {
-        sm_m[warp * ROWS + nt * 8 + 2 * c + e] = m[nt][e];
-        sm_l[warp * ROWS + nt * 8 + 2 * c + e] = l[nt][e];
-      }
-    }
-  __syncthreads();
-  float lt[NT][2], mt[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = nt * 8 + 2 * c + e;
-      float mx = kNoMax;
-#pragma unroll
-      for (int w = 0; w < W; ++w) mx = fmaxf(mx, sm_m[w * ROWS + r]);
-      float sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) sum = fmaf(sm_l[w * ROWS + r], fast_exp2((sm_m[w * ROWS + r] - mx) * sl), sum);
-      const float alpha = fast_exp2((m[nt][e] - mx) * sl);
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) acc[d][nt][e] *= alpha, acc[d][nt][e + 2] *= alpha;
-      lt[nt][e] = sum, mt[nt][e] = mx;
-    }
-  float* tree = reinterpret_cast<float*>(smem);
-  constexpr int kVals = D / 16 * NT * 4;
-#pragma unroll
-  for (int half = W / 2; half >= 1; half >>= 1) {
-    if (warp >= half && warp < 2 * half) {
-#pragma unroll
-      for (int x = 0; x < kVals; ++x)
-        tree[((warp - half) * kVals + x) * 32 + lane] = acc[x / (NT * 4)][(x / 4) % NT][x % 4];
-    }
-    __syncthreads();
-    if (warp < half) {
-#pragma unroll
-      for (int x = 0; x < kVals; ++x)
-        acc[x / (NT * 4)][(x / 4) % NT][x % 4] += tree[(warp * kVals + x) * 32 + lane];
-    }
-    __syncthreads();
-  }
-  if (warp != 0) return;
-  const bool whole = rg.tiles <= split_tiles;   // no other split has keys: the result is final
+  // ---- the run's result: rows 2c, 2c + 1 of every eight, channels g8 * D/8 + x
+  const bool whole = rg.tiles <= split_tiles;   // no other run has keys: the result is final
+  const float unit = MX ? pow2(v_ref - 127) : 1.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = nt * 8 + 2 * c + e;
       if (r >= row_count) continue;
-      float f[D / 8];   // channels g8 * D/8 + x
+      const float sum = l[nt][e];
+      float f[D / 8];
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) f[2 * d] = acc[d][nt][e], f[2 * d + 1] = acc[d][nt][e + 2];
+      for (int d = 0; d < D / 16; ++d) f[2 * d] = acc[d][nt][e] * unit, f[2 * d + 1] = acc[d][nt][e + 2] * unit;
       if (whole) {
         const int t = (r0 + r) / G, h = kvh * G + (r0 + r) % G;
         // rows behind the sequence's last new token, and rows that see nothing, are zero
-        const float inv = (r0 + r) < rg.n * G && lt[nt][e] > 0.0f ? 1.0f / lt[nt][e] : 0.0f;
-        const bool nan = !(lt[nt][e] >= 0.0f);
+        const bool zero = (r0 + r) >= rg.n * G || sum == 0.0f;
+        const float inv = 1.0f / sum;
         __nv_bfloat16* dst = a.out + ((static_cast<long long>(b) * a.T + t) * a.H + h) * D + g8 * (D / 8);
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) {
           uint32_t w[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float v0 = f[8 * x + 2 * y], v1 = f[8 * x + 2 * y + 1];
-            w[y] = (r0 + r) >= rg.n * G ? 0u : nan ? 0x7fc07fc0u : inv == 0.0f ? 0u : pack_bf16(v0 * inv, v1 * inv);
-          }
+          for (int y = 0; y < 4; ++y) w[y] = zero ? 0u : pack_bf16(f[8 * x + 2 * y] * inv, f[8 * x + 2 * y + 1] * inv);
           *reinterpret_cast<uint4*>(dst + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       } else {
@@ -535,43 +557,45 @@ __global__ void __launch_bounds__(Ring<D, MX>::kWarps * 32, NT == 1 ? 2 : 1) pag
         float4* dst = reinterpret_cast<float4*>(a.part_o + (at * rw + r) * D + g8 * (D / 8));
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) dst[x] = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
-        if (g8 == 0) {
-          a.part_ml[(at * rw + r) * 2] = mt[nt][e] * sl;
-          a.part_ml[(at * rw + r) * 2 + 1] = lt[nt][e];
-        }
+        if (g8 == 0) *reinterpret_cast<float2*>(a.part_ml + (at * rw + r) * 2) = make_float2(m[nt][e], sum);
       }
     }
 }
 
-// One warp per output row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). Rows that one split finished are skipped.
+// One CTA per output row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). Its warps take the runs in turn. Rows that
+// one run finished are skipped.
+constexpr int kCombineWarps = 4;
 template <int D>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a, int rows) {
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedAttnArgs a, int rows) {
+  __shared__ float sm_o[kCombineWarps][D], sm_l[kCombineWarps], sm_m[kCombineWarps];
   NC_PDL_PROLOGUE();
-  const int G = a.H / a.KV, lane = threadIdx.x & 31;
-  const long long total = static_cast<long long>(a.B) * a.KV * a.T * G;
-  const long long id = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (id >= total) return;
-  const int r = static_cast<int>(id % (a.T * G));
-  const int kvh = static_cast<int>(id / (a.T * G) % a.KV), b = static_cast<int>(id / (static_cast<long long>(a.T) * G * a.KV));
+  const int G = a.H / a.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = a.T * G;
+  const int r = static_cast<int>(blockIdx.x % per);
+  const int kvh = static_cast<int>(blockIdx.x / per % a.KV), b = static_cast<int>(blockIdx.x / per / a.KV);
   const int rb = r / rows;
   const Range rg = range_of(a, b, rb * rows, rows);
   const int split_tiles = a.split_keys / kTile;
   if (rg.tiles <= split_tiles) return;
   const bool real = r < rg.n * G;   // a row behind the last new token is zero
-  const int n = (rg.tiles + split_tiles - 1) / split_tiles;
-  const int rw = min(rows, a.T * G);
-  const long long blocks = static_cast<long long>(a.KV) * ((a.T * G + rows - 1) / rows);
+  const int n = real ? (rg.tiles + split_tiles - 1) / split_tiles : 0;
+  const int rw = min(rows, per);
+  const long long blocks = static_cast<long long>(a.KV) * ((per + rows - 1) / rows);
   const long long at = ((static_cast<long long>(b) * blocks + rb * a.KV + kvh) * a.splits) * rw + (r - rb * rows);
   float mx = -CUDART_INF_F;
-  for (int s = lane; real && s < n; s += 32) mx = fmaxf(mx, a.part_ml[(at + static_cast<long long>(s) * rw) * 2]);
+  for (int s = threadIdx.x; s < n; s += kCombineWarps * 32) mx = fmaxf(mx, a.part_ml[(at + static_cast<long long>(s) * rw) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) sm_m[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) mx = fmaxf(mx, sm_m[w]);
   constexpr int E = D / 32;
   float o[E], ls = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll 4
-  for (int s = 0; real && s < n; ++s) {
+  for (int s = warp; s < n; s += kCombineWarps) {
     const long long p = at + static_cast<long long>(s) * rw;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
     const float w = fast_exp2(ml.x - mx);
@@ -584,16 +608,18 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
       o[0] = fmaf(w, x.x, o[0]), o[1] = fmaf(w, x.y, o[1]);
     }
   }
-  const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-  if (!real) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-  }
+  for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
+  if (lane == 0) sm_l[warp] = ls;
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  float x = 0.0f, y = 0.0f;
+  ls = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) x += sm_o[w][2 * threadIdx.x], y += sm_o[w][2 * threadIdx.x + 1], ls += sm_l[w];
+  const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
   __nv_bfloat16* dst = a.out + ((static_cast<long long>(b) * a.T + r / G) * a.H + kvh * G + r % G) * D;
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_bf16(o[0] * inv, o[1] * inv);
+  reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = real ? pack_bf16(x * inv, y * inv) : 0u;
 }
 
 // Rows per CTA: the query rows of a kv head in blocks of 8, 16 or 32.
@@ -604,24 +630,24 @@ int row_tiles(const PagedAttnArgs& a) {
 
 template <int D, bool MX, int NT, bool P16>
 cudaError_t launch_rows(const PagedAttnArgs& a, cudaStream_t s) {
-  using L = RowsSmem<D, MX, NT>;
+  using R = Ring<D, MX>;
+  constexpr int ROWS = 8 * NT;
   static std::atomic<unsigned long long> configured{0};   // one bit per device
   int dev = 0;
   cudaGetDevice(&dev);
   const unsigned long long bit = 1ull << (dev & 63);
   if ((configured.load(std::memory_order_relaxed) & bit) == 0) {
     const cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<D, MX, NT, P16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               L::kTotal);
+                                               R::kBytes);
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit);
   }
-  const int G = a.H / a.KV, blocks = (a.T * G + L::kRows - 1) / L::kRows;
-  cudaError_t e = launch_maybe_pdl(paged_rows_kernel<D, MX, NT, P16>, dim3(a.splits, a.KV * blocks, a.B),
-                                   dim3(Ring<D, MX>::kWarps * 32), L::kTotal, s, a);
+  const int G = a.H / a.KV, blocks = (a.T * G + ROWS - 1) / ROWS;
+  cudaError_t e = launch_maybe_pdl(paged_rows_kernel<D, MX, NT, P16>, dim3(a.splits, a.KV * blocks, a.B), dim3(32), R::kBytes, s, a);
   if (e != cudaSuccess || a.splits <= 1) return e;
-  const long long total = static_cast<long long>(a.B) * a.T * a.H;
-  return launch_maybe_pdl(paged_combine_kernel<D>, dim3(static_cast<unsigned>((total + 3) / 4)), dim3(128), 0, s, a,
-                          static_cast<int>(L::kRows));
+  // always behind the first kernel's tail (it waits for it before it reads anything)
+  return launch_pdl(true, paged_combine_kernel<D>, dim3(static_cast<unsigned>(static_cast<long long>(a.B) * a.T * a.H)),
+                    dim3(kCombineWarps * 32), 0, s, a, static_cast<int>(ROWS));
 }
 template <int D, bool MX>
 cudaError_t launch_shape(const PagedAttnArgs& a, cudaStream_t s) {
@@ -638,20 +664,19 @@ cudaError_t launch_shape(const PagedAttnArgs& a, cudaStream_t s) {
 }  // namespace
 
 PagedPlan paged_rows_plan(const PagedAttnArgs& a) {
-  const bool mx = a.k_scale != nullptr;
   const int G = a.H / a.KV, rows = 8 * row_tiles(a), blocks = (a.T * G + rows - 1) / rows;
-  const int step = kTile * (mx ? 8 : 4);   // keys that one CTA's warps take at a time
   long long keys = static_cast<long long>(a.max_pages) * a.page_size;
   if (a.window_left >= 0) keys = std::min(keys, static_cast<long long>(a.window_left) + 1 + (rows + G - 1) / G);
   const long long units = static_cast<long long>(a.B) * a.KV * blocks;
-  // Two CTAs per SM, twice over, so that sequences of different lengths even out; never less than one step per CTA.
-  const long long want = 148 * 4;
+  // Runs that fill the warps of two CTAs per SM about three times over (so that the last ones even out), of 64 keys at
+  // least (below that the fixed cost of a run and of joining it outweighs the keys) and kMaxRun at most.
+  const long long want = 148LL * 16 * 3;
   long long per = (keys * units + want - 1) / want;
-  per = std::min<long long>((per + step - 1) / step * step, 4096);
+  per = (std::min<long long>(std::max<long long>(per, 64), kMaxRun) + kTile - 1) / kTile * kTile;
   PagedPlan p;
-  p.split_keys = static_cast<int>(std::max<long long>(per, step));
+  p.split_keys = static_cast<int>(per);
   // a range that starts inside a tile touches one tile more
-  p.splits = static_cast<int>(((keys + kTile - 1) / kTile + 1 + p.split_keys / kTile - 1) / (p.split_keys / kTile));
+  p.splits = static_cast<int>(((keys + kTile - 1) / kTile + 1 + per / kTile - 1) / (per / kTile));
   if (p.splits > 1) {
     const long long rw = std::min<long long>(rows, static_cast<long long>(a.T) * G);
     p.part_o = units * p.splits * rw * a.D;
