@@ -1,0 +1,578 @@
+// Attention of a chunk of new tokens over the paged cache (bf16 or MXFP8 pages): many rows per kv head, on tcgen05.
+//
+// Rows are (query token, head of the group): the heads that share a kv head are packed into the 128-row tiles of one CTA
+// (the largest power of two that divides the group), so keys and values are read once for all of them and a chunk
+// of a few tokens still fills a tile. A CTA takes two such tiles and walks the keys that either sees, 64 at a time:
+//   warps 0..3, 4..7  softmax of row tile 0 and 1: a thread owns a row; P replaces S in tensor memory as bf16
+//   warp 8            tcgen05.mma: S^x = Q^x K^T (two buffers per tile), O^x += P^x V, O in tensor memory all along
+//   warp 9            TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
+//   warps 10..13      on MXFP8 pages: codes are read from global memory one tile ahead, spread to bf16, multiplied by
+//                     their block's power of two (exact) and stored in the operands' 128-byte swizzled layout
+// A page that is not in the pool, and 16 tokens that no row sees, become rows of zeros; values of the first and last
+// 16 tokens that are only partly seen are copied by hand with zeros in the unseen places, because what lies there
+// (a place behind the sequence's end) may be NaN, and 0 * NaN is not 0.
+// The running maximum is raised only when a tile exceeds it by more than 2^8: then the thread rescales its O row in tensor
+// memory. Bound by the exponentials (16 a clock and SM: 512 clocks per 128 x 64 tile, against 256 for its products).
+// grid: (blocks of 256 rows x key runs, kv heads x head packs, sequences), the blocks that see most first.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <math_constants.h>
+
+#include <atomic>
+
+#include "mx_cache.cuh"
+#include "paged_common.cuh"
+#include "ptx.cuh"
+#include "serving.h"
+#include "tmap.h"
+
+namespace nc {
+
+namespace {
+
+constexpr int BQ = 128;    // rows per tile (TMEM lanes)
+constexpr int NQ = 2;      // row tiles per CTA
+constexpr int BKV = 64;    // keys per step
+constexpr int KVS = 3;     // stages of K and of V
+constexpr int kBox = 16;   // tokens per TMA box: a page holds a multiple of it
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+template <int D, bool MX>
+struct ChunkLayout {
+  static constexpr int kQ = BQ * D * 2;
+  static constexpr int kKV = BKV * D * 2;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + NQ * kQ;
+  static constexpr int kOffV = kOffK + KVS * kKV;
+  static constexpr int kOffBar = kOffV + KVS * kKV;
+  static constexpr int kTotal = kOffBar + 512 + 1024;
+  static constexpr int kThreads = (NQ * 4 + 2 + (MX ? 4 : 0)) * 32;
+};
+
+struct ChunkParams {
+  PagedAttnArgs a;   // a.KV counts packs of heads, a.H / a.KV heads each
+  int kv_per_pack;   // real kv head = pack / kv_per_pack
+  int KV;            // real kv heads
+};
+
+template <int D, bool MX>
+__global__ void __launch_bounds__(ChunkLayout<D, MX>::kThreads, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const ChunkParams p) {
+  using L = ChunkLayout<D, MX>;
+  constexpr int DC = D / 64;
+  const PagedAttnArgs& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* q_full = bars + 0;
+  uint64_t* k_full = bars + 1;
+  uint64_t* k_empty = k_full + KVS;
+  uint64_t* v_full = k_empty + KVS;
+  uint64_t* v_empty = v_full + KVS;
+  uint64_t* tile_bars = v_empty + KVS;   // per row tile: s_full[2], s_empty[2], p_full[2], o_done, o_final
+  auto s_full = [&](int x, int i) { return tile_bars + 8 * x + i; };
+  auto s_empty = [&](int x, int i) { return tile_bars + 8 * x + 2 + i; };
+  auto p_full = [&](int x, int i) { return tile_bars + 8 * x + 4 + i; };
+  auto o_done = [&](int x) { return tile_bars + 8 * x + 6; };    // flips after every P V product
+  auto o_final = [&](int x) { return tile_bars + 8 * x + 7; };   // once, after the last
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tile_bars + 8 * NQ);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.H / a.KV;                               // heads in a pack: a power of two
+  const int blocks = (a.T * G + NQ * BQ - 1) / (NQ * BQ);
+  const int qb = blocks - 1 - static_cast<int>(blockIdx.x) / a.splits, split = blockIdx.x % a.splits;
+  const int pack = blockIdx.y, kvh = pack / p.kv_per_pack, b = blockIdx.z;
+  const int r0 = qb * NQ * BQ, row_count = min(NQ * BQ, a.T * G - r0);
+  const Range rg = range_of(a, b, r0, NQ * BQ, BKV);
+  const int split_tiles = a.split_keys / BKV;
+  const bool whole = rg.tiles <= split_tiles;             // no other run has keys: the result is final
+  const int first = rg.tile0 + split * split_tiles;
+  const int n_u = min(rg.tiles - split * split_tiles, split_tiles);   // key tiles of this CTA
+  if (split > 0 && n_u <= 0) return;
+  if (split == 0 && threadIdx.x == 0 && rg.pmax >= static_cast<long long>(a.max_pages) * a.page_size && a.status != nullptr)
+    atomicCAS(a.status, 0, kErrBadIndex);   // keys past the page table are left out
+  auto out_row = [&](int r) {   // row r of the block
+    return a.out + ((static_cast<long long>(b) * a.T + (r0 + r) / G) * a.H + pack * G + (r0 + r) % G) * D;
+  };
+  if (n_u <= 0) {               // nothing is seen: zeros
+    for (int i = threadIdx.x; i < row_count * (D / 8); i += L::kThreads)
+      reinterpret_cast<uint4*>(out_row(i / (D / 8)))[i % (D / 8)] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  // key tiles of each row tile inside this CTA's run
+  int lo[NQ], hi[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const Range t = range_of(a, b, r0 + x * BQ, BQ, BKV);
+    lo[x] = max(t.tile0, first);
+    hi[x] = t.tiles > 0 ? min(t.tile0 + t.tiles - 1, first + n_u - 1) : -1;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < KVS; ++i) {
+      mbar_init(&k_full[i], MX ? 4 : 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], MX ? 4 : 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int x = 0; x < NQ; ++x) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full(x, i), 1);
+        mbar_init(s_empty(x, i), 4);
+        mbar_init(p_full(x, i), 4);
+      }
+      mbar_init(o_done(x), 1);
+      mbar_init(o_final(x), 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == NQ * 4) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  const int* table = a.page_table + static_cast<long long>(b) * a.max_pages;
+  // A page that is none of the pool's is found here once; only then are pages looked at again where scores are masked.
+  bool bad = false;
+  for (int pg = max(first * BKV, rg.lo) / a.page_size + threadIdx.x; pg <= (min((first + n_u) * BKV, rg.hi) - 1) / a.page_size;
+       pg += L::kThreads) {
+    const int page = table[pg];
+    bad = bad || page < 0 || page >= a.num_pages;
+  }
+  if (bad && a.status != nullptr) atomicCAS(a.status, 0, kErrBadIndex);
+  tc_fence_before();
+  const bool any_bad = __syncthreads_or(bad);
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  auto tmem_S = [&](int x, int buf) { return tmem_base + x * 128 + buf * BKV; };
+  auto tmem_O = [&](int x) { return tmem_base + 256 + x * 128; };
+
+  if (warp == NQ * 4) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc_bf16(BQ, BKV, false, false);
+      constexpr uint32_t idesc_o = make_idesc_bf16(BQ, D, false, true);
+      const uint64_t q_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 16, 1024);
+      const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 16, 1024);
+      const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffV), BKV * 128, 1024);
+      auto issue_s = [&](int s) -> bool {
+        const int j = first + s, st = s % KVS;
+        if (!mbar_wait(&k_full[st], (s / KVS) & 1, abort_flag, a.status, kErrWaitFull)) return false;
+        const uint64_t dk = k_desc0 + static_cast<uint64_t>(st * (L::kKV >> 4));
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if (j < lo[x] || j > hi[x]) continue;
+          const int i = j - lo[x];
+          if (!mbar_wait(s_empty(x, i & 1), ((i >> 1) & 1) ^ 1, abort_flag, a.status, kErrWaitTmemEmpty)) return false;
+          tc_fence_after();
+          const uint64_t dq = q_desc0 + static_cast<uint64_t>(x * (L::kQ >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t qo = static_cast<uint64_t>(((k / 4) * (BQ * 128) + (k % 4) * 32) >> 4);
+            const uint64_t ko = static_cast<uint64_t>(((k / 4) * (BKV * 128) + (k % 4) * 32) >> 4);
+            mma_f16_ss(tmem_S(x, i & 1), dq + qo, dk + ko, idesc_s, k > 0 ? 1u : 0u);
+          }
+          mma_commit(s_full(x, i & 1));
+        }
+        mma_commit(&k_empty[st]);
+        return true;
+      };
+      auto issue_o = [&](int s) -> bool {
+        const int j = first + s, st = s % KVS;
+        if (!mbar_wait(&v_full[st], (s / KVS) & 1, abort_flag, a.status, kErrWaitFull)) return false;
+        const uint64_t dv = v_desc0 + static_cast<uint64_t>(st * (L::kKV >> 4));
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if (j < lo[x] || j > hi[x]) continue;
+          const int i = j - lo[x];
+          if (!mbar_wait(p_full(x, i & 1), (i >> 1) & 1, abort_flag, a.status, kErrWaitOther)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < BKV / 16; ++k)
+            mma_f16_ts(tmem_O(x), tmem_S(x, i & 1) + k * 8, dv + static_cast<uint64_t>((k * 16 * 128) >> 4), idesc_o,
+                       (i > 0 || k > 0) ? 1u : 0u);
+          mma_commit(o_done(x));
+          if (j == hi[x]) mma_commit(o_final(x));
+        }
+        mma_commit(&v_empty[st]);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0, abort_flag, a.status, kErrWaitFull);
+      for (int s = 0; s <= n_u && ok; ++s) {
+        if (s < n_u) ok = issue_s(s);
+        if (ok && s >= 1) ok = issue_o(s - 1);
+      }
+    }
+  } else if (warp == NQ * 4 + 1) {
+    // ---------------------------------------------------------------- TMA: Q, and bf16 keys and values
+    if (lane == 0) {
+      mbar_expect_tx(q_full, NQ * L::kQ);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x)
+#pragma unroll
+        for (int c = 0; c < DC; ++c)   // tokens past T are read as zeros
+          tma_load_4d(smem + L::kOffQ + x * L::kQ + c * (BQ * 128), &tmQ, q_full, c * 64, pack * G, (r0 + x * BQ) / G, b);
+    }
+    bool ok = true;
+    if constexpr (!MX) {
+      const int out_of_pool = a.num_pages * a.page_size;   // a row outside the map: the box arrives as zeros
+      int st = 0;
+      uint32_t ph = 0;
+      for (int s = 0; s < n_u && ok; ++s) {
+        // lanes 0..3: the four boxes of the tile
+        const int key = (first + s) * BKV + (lane & 3) * kBox;
+        int row = out_of_pool;
+        bool partial = false;
+        if (key + kBox > rg.lo && key < rg.hi) {
+          const int page = table[key / a.page_size];
+          if (page >= 0 && page < a.num_pages) row = page * a.page_size + key % a.page_size;
+          partial = row != out_of_pool && (key < rg.lo || key + kBox > rg.hi);
+        }
+        const unsigned by_hand = __ballot_sync(0xffffffffu, partial && lane < 4);
+        ok = mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        uint8_t* sk = smem + L::kOffK + st * L::kKV;
+        uint8_t* sv = smem + L::kOffV + st * L::kKV;
+        if (lane == 0) mbar_expect_tx(&k_full[st], L::kKV);
+        __syncwarp();
+        if (lane < 4)
+#pragma unroll
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sk + c * (BKV * 128) + lane * (kBox * 128), &tmK, &k_full[st], c * 64, row, kvh);
+        __syncwarp();
+        ok = mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (by_hand != 0) {
+          for (int box = 0; box < 4; ++box) {
+            if (((by_hand >> box) & 1) == 0) continue;
+            const int row_b = __shfl_sync(0xffffffffu, row, box), key_b = (first + s) * BKV + box * kBox;
+            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.v_pool) +
+                                       (static_cast<long long>(row_b) * p.KV + kvh) * D;
+            for (int i = lane; i < kBox * (D / 8); i += 32) {
+              const int t = i / (D / 8), u = i % (D / 8);
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if (key_b + t >= rg.lo && key_b + t < rg.hi)
+                w = *reinterpret_cast<const uint4*>(src + static_cast<long long>(t) * p.KV * D + u * 8);
+              *reinterpret_cast<uint4*>(sv + (u >> 3) * (BKV * 128) + (box * kBox + t) * 128 + (((u & 7) ^ (t & 7)) * 16)) = w;
+            }
+          }
+          fence_async_shared();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_expect_tx(&v_full[st], L::kKV - __popc(by_hand) * kBox * D * 2);
+        __syncwarp();
+        if (lane < 4 && !partial)
+#pragma unroll
+          for (int c = 0; c < DC; ++c)
+            tma_load_3d(sv + c * (BKV * 128) + lane * (kBox * 128), &tmV, &v_full[st], c * 64, row, kvh);
+        if (++st == KVS) { st = 0; ph ^= 1; }
+      }
+    }
+    if (!ok) {   // copies in flight land before the CTA ends
+      const unsigned long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+  } else if (MX && warp >= NQ * 4 + 2) {
+    // ---------------------------------------------------------------- MXFP8 keys and values -> bf16 operands
+    if constexpr (MX) {
+      constexpr int U = D / 16;                 // 16-code pieces of a row
+      constexpr int N = BKV * U / 128;          // pieces per thread and side: rows t / U + i * (128 / U)
+      constexpr int kRows = 128 / U;
+      const int t = threadIdx.x - (NQ * 4 + 2) * 32;
+      const int row0 = t / U, u = t % U;
+      const uint8_t *kp = static_cast<const uint8_t*>(a.k_pool), *vp = static_cast<const uint8_t*>(a.v_pool);
+      uint4 kc[N], vc[N];
+      uint32_t kb[N], vb[N];
+      auto fetch = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int key = (first + s) * BKV + row0 + i * kRows;
+          kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
+          kb[i] = vb[i] = 127;
+          if (key < rg.lo || key >= rg.hi) continue;
+          const int page = table[key / a.page_size], slot = key % a.page_size;
+          if (page < 0 || page >= a.num_pages) continue;
+          const long long at = ((static_cast<long long>(page) * a.page_size + slot) * p.KV + kvh) * D + u * 16;
+          const long long sc = ((static_cast<long long>(page) * p.KV + kvh) * a.page_size + slot) * (D / 32) + u / 2;
+          kc[i] = *reinterpret_cast<const uint4*>(kp + at);
+          vc[i] = *reinterpret_cast<const uint4*>(vp + at);
+          kb[i] = a.k_scale[sc];
+          vb[i] = a.v_scale[sc];
+        }
+      };
+      auto store = [&](uint8_t* base, const uint4 (&code)[N], const uint32_t (&sb)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = row0 + i * kRows;
+          const uint32_t f1 = mx_factor_first(sb[i]) * 0x10001u, f2 = mx_factor_second(sb[i]) * 0x10001u;
+          const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            mx_spread(w[y], o[2 * y], o[2 * y + 1]);
+            o[2 * y] = mul_bf16x2(o[2 * y], f1), o[2 * y + 1] = mul_bf16x2(o[2 * y + 1], f1);
+          }
+          if (sb[i] > 134u) {
+#pragma unroll
+            for (int y = 0; y < 8; ++y) o[y] = mul_bf16x2(o[y], f2);
+          }
+          uint8_t* row = base + (u >> 2) * (BKV * 128) + r * 128;
+          const int g = (u & 3) * 2;
+          *reinterpret_cast<uint4*>(row + ((g ^ (r & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row + (((g + 1) ^ (r & 7)) * 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_async_shared();
+        __syncwarp();
+      };
+      int st = 0;
+      uint32_t ph = 0;
+      fetch(0);
+      for (int s = 0; s < n_u; ++s) {
+        if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty)) break;
+        store(smem + L::kOffK + st * L::kKV, kc, kb);
+        if (lane == 0) mbar_arrive(&k_full[st]);
+        if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty)) break;
+        store(smem + L::kOffV + st * L::kKV, vc, vb);
+        if (s + 1 < n_u) fetch(s + 1);
+        if (lane == 0) mbar_arrive(&v_full[st]);
+        if (++st == KVS) { st = 0; ph ^= 1; }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int x = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int r = r0 + x * BQ + row;             // row of the pack
+    const bool row_in = x * BQ + row < row_count, real = r < rg.n * G;
+    const int qpos = real ? rg.base + r / G : -1;
+    const int t_last = min((r0 + x * BQ + BQ - 1) / G, rg.n - 1);
+    const int pos_min = rg.base + (r0 + x * BQ) / G, pos_max = rg.base + t_last;   // of the tile's real rows
+    const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int n_x = hi[x] - lo[x] + 1;
+    const float sl = a.scale * 1.4426950408889634f;
+    float m_ref = -1.0e30f, l_run = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < n_x && ok; ++i) {
+      const int sb = i & 1;
+      const int kv0 = (lo[x] + i) * BKV;
+      const bool need_mask = any_bad || kv0 + BKV - 1 > pos_min || (a.window_left >= 0 && kv0 < pos_max - a.window_left) || kv0 + BKV > rg.hi;
+      if (!mbar_wait(s_full(x, sb), (i >> 1) & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t r0v[32], r1v[32];
+      tmem_ld_32x32(tmem_S(x, sb) + lane_sel, r0v);
+      tmem_ld_32x32(tmem_S(x, sb) + 32 + lane_sel, r1v);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_empty(x, sb));
+      float sv[64];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sv[e] = __uint_as_float(r0v[e]), sv[32 + e] = __uint_as_float(r1v[e]);
+      if (need_mask) {
+        // keys [k_lo, k_hi) of this tile are seen by the row; the rest cannot be told from seen ones by value
+        const int k_hi = min(qpos + 1, rg.hi) - kv0, k_lo = (a.window_left >= 0 ? max(0, qpos - a.window_left) : 0) - kv0;
+#pragma unroll
+        for (int e = 0; e < 64; ++e) sv[e] = e >= k_lo && e < k_hi ? sv[e] : -CUDART_INF_F;
+        for (int box = 0; any_bad && box < BKV / kBox; ++box) {   // a page outside the pool: its keys are none
+          const int key = kv0 + box * kBox;
+          if (key >= rg.hi || key + kBox <= rg.lo) continue;
+          const int page = table[key / a.page_size];
+          if (page < 0 || page >= a.num_pages) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) sv[e] = (e >> 4) == box ? -CUDART_INF_F : sv[e];
+          }
+        }
+      }
+      float m_tile = -1.0e30f;
+#pragma unroll
+      for (int e = 0; e < 64; ++e) m_tile = fmaxf(m_tile, sv[e]);
+      const bool raise = (m_tile - m_ref) * sl > kRescaleThreshold;
+      if (__any_sync(0xffffffffu, raise)) {
+        float alpha = 1.0f;
+        if (raise) {
+          alpha = fast_exp2((m_ref - m_tile) * sl);
+          m_ref = m_tile;
+          l_run *= alpha;
+        }
+        if (i > 0) {
+          if (!mbar_wait(o_done(x), (i - 1) & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem_O(x) + c * 16 + lane_sel, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x16(tmem_O(x) + c * 16 + lane_sel, o);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+        }
+      }
+      const float m_scaled = m_ref * sl;
+      uint32_t packed[32];
+      float l_tile = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const uint32_t pk = pack_bf16(fast_exp2(sv[e] * sl - m_scaled), fast_exp2(sv[e + 1] * sl - m_scaled));
+        l_tile += bf16_lo(pk) + bf16_hi(pk);
+        packed[e / 2] = pk;
+      }
+      l_run += l_tile;
+      tmem_st_32x32(tmem_S(x, sb) + lane_sel, packed);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(x, sb));
+    }
+    if (ok && n_x > 0) ok = mbar_wait(o_final(x), 0, abort_flag, a.status, kErrWaitTmemFull);
+    if (ok) {
+      tc_fence_after();
+      const bool any = n_x > 0;                 // else O was never written
+      if (whole) {
+        const bool zero = !any || !real || l_run == 0.0f;
+        const float inv_l = 1.0f / l_run;
+        __nv_bfloat16* op = out_row(x * BQ + (row_in ? row : 0));
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t w[32];
+          if (any) {
+            tmem_ld_32x32(tmem_O(x) + c * 32 + lane_sel, w);
+            tmem_ld_wait();
+          }
+          if (row_in) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                y[e] = zero ? 0u : pack_bf16(__uint_as_float(w[g * 8 + e * 2]) * inv_l, __uint_as_float(w[g * 8 + e * 2 + 1]) * inv_l);
+              *reinterpret_cast<uint4*>(op + c * 32 + g * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+        }
+      } else {
+        const int rw = min(NQ * BQ, a.T * G);
+        const long long at = ((static_cast<long long>(b) * gridDim.y * blocks + static_cast<long long>(qb) * gridDim.y + pack) *
+                                  a.splits + split) * rw + x * BQ + row;
+        float* dst = a.part_o + at * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t w[32];
+          if (any) {
+            tmem_ld_32x32(tmem_O(x) + c * 32 + lane_sel, w);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = 0;
+          }
+          if (row_in) {
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              *reinterpret_cast<uint4*>(dst + c * 32 + g * 4) = make_uint4(w[g * 4], w[g * 4 + 1], w[g * 4 + 2], w[g * 4 + 3]);
+          }
+        }
+        if (row_in) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref * sl, any ? l_run : 0.0f);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NQ * 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Heads per pack: the largest power of two (at most a tile) that divides the group.
+int pack_of(int G) {
+  int p = 1;
+  while (p < BQ && G % (2 * p) == 0) p *= 2;
+  return p;
+}
+
+template <int D, bool MX>
+const char* launch_chunk(const PagedAttnArgs& args, cudaStream_t s) {
+  using L = ChunkLayout<D, MX>;
+  ChunkParams p;
+  p.a = args;
+  const int G = args.H / args.KV, P = pack_of(G);
+  p.KV = args.KV;
+  p.kv_per_pack = G / P;
+  p.a.KV = args.H / P;
+  CUtensorMap tq, tk, tv;
+  const long long dq[4] = {D, args.H, args.T, args.B};
+  const long long sq[3] = {args.q_stride_h, args.q_stride_t, args.q_stride_b};
+  const int boxq[4] = {64, P, BQ / P, 1};
+  if (!make_tmap_bf16_4d(&tq, args.q, dq, sq, boxq)) return "paged_chunk_attention: tensor map construction failed";
+  tk = tv = tq;
+  if (!MX) {
+    const long long rows = static_cast<long long>(args.num_pages) * args.page_size, stride = static_cast<long long>(args.KV) * D;
+    if (!make_tmap_bf16_3d(&tk, args.k_pool, D, rows, args.KV, stride, D, 64, kBox) ||
+        !make_tmap_bf16_3d(&tv, args.v_pool, D, rows, args.KV, stride, D, 64, kBox))
+      return "paged_chunk_attention: tensor map construction failed";
+  }
+  static std::atomic<unsigned long long> configured{0};   // one bit per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if ((configured.load(std::memory_order_relaxed) & bit) == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_chunk_kernel<D, MX>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
+    configured.fetch_or(bit);
+  }
+  const int blocks = (args.T * P + NQ * BQ - 1) / (NQ * BQ);
+  const dim3 grid(static_cast<unsigned>(blocks) * args.splits, p.a.KV, args.B);
+  paged_chunk_kernel<D, MX><<<grid, L::kThreads, L::kTotal, s>>>(tq, tk, tv, p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && args.splits > 1) e = launch_combine<D>(p.a, NQ * BQ, BKV, s);
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
+
+}  // namespace
+
+PagedPlan paged_chunk_plan(const PagedAttnArgs& a) {
+  const int P = pack_of(a.H / a.KV), rows = NQ * BQ, blocks = (a.T * P + rows - 1) / rows;
+  long long keys = static_cast<long long>(a.max_pages) * a.page_size;
+  if (a.window_left >= 0) keys = std::min(keys, static_cast<long long>(a.window_left) + 1 + rows / P);
+  const long long units = static_cast<long long>(a.B) * (a.H / P) * blocks;
+  // One CTA per SM: four waves of them, so that the last one is a small part; runs of 512 keys at least (joining a run
+  // costs as much as some 100 keys).
+  const long long want = (148 * 4 + units - 1) / units;
+  long long per = ((keys + want - 1) / want + BKV - 1) / BKV * BKV;
+  per = std::max<long long>(per, 512);
+  PagedPlan p;
+  p.split_keys = static_cast<int>(std::min<long long>(per, 1 << 30));
+  // a window may start inside a tile and touch one more
+  p.splits = static_cast<int>(((keys + BKV - 1) / BKV + (a.window_left >= 0 ? 1 : 0) + per / BKV - 1) / (per / BKV));
+  if (want == 1) p.splits = 1, p.split_keys = 1 << 30;
+  if (p.splits > 1) {
+    const long long rw = std::min<long long>(rows, static_cast<long long>(a.T) * P);
+    p.part_o = units * p.splits * rw * a.D;
+    p.part_ml = units * p.splits * rw * 2;
+  }
+  return p;
+}
+
+bool paged_chunk_takes(const PagedAttnArgs& a) {
+  // Few rows per kv head leave most of a 128-row tile empty: the other kernel reads the keys at full speed. TMA boxes
+  // are 16 tokens of one page. A scale that is not positive turns the maximum around.
+  const int P = pack_of(a.H / a.KV);
+  return a.T * (a.H / a.KV) > 16 && a.page_size % kBox == 0 && a.scale > 0.0f && a.H / P <= 65535 &&
+         static_cast<long long>(a.num_pages) * a.page_size < (1LL << 31) - 1024;
+}
+
+const char* paged_chunk_attention(const PagedAttnArgs& a, cudaStream_t s) {
+  if (a.B == 0 || a.T == 0) return nullptr;
+  if (a.splits > 1 && (a.part_o == nullptr || a.part_ml == nullptr)) return "paged attention: no workspace for the key splits";
+  const bool mx = a.k_scale != nullptr;
+  if (a.D == 128) return mx ? launch_chunk<128, true>(a, s) : launch_chunk<128, false>(a, s);
+  return mx ? launch_chunk<64, true>(a, s) : launch_chunk<64, false>(a, s);
+}
+
+}  // namespace nc

@@ -27,6 +27,7 @@
 
 #include "host_build.h"
 #include "mx_cache.cuh"
+#include "paged_common.cuh"
 #include "pdl_launch.h"
 #include "ptx.cuh"
 #include "serving.h"
@@ -41,11 +42,6 @@ constexpr int kMaxRun = 512;     // keys of one warp's run at most: its page num
 constexpr float kRaise = 8.0f;   // log2 units
 constexpr float kNoMax = -1.0e30f;
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 template <bool F16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (F16)
@@ -100,32 +96,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// What the rows [r0, r0 + rows) of sequence b see: row r is query token r / G, head r % G of the kv head's group.
-struct Range {
-  int n;             // new tokens of the sequence
-  int base;          // position of its first new token
-  int pmin, pmax;    // positions of the block's first and last real row
-  int lo, hi;        // keys [lo, hi) that some row sees; hi <= lo: none
-  int tile0, tiles;  // 16-key tiles that cover them
-};
-__device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int b, int r0, int rows) {
-  Range g;
-  const int G = a.H / a.KV, len = a.seq_lens[b];
-  g.n = a.q_lens != nullptr ? min(max(a.q_lens[b], 0), a.T) : a.T;
-  g.base = len - g.n;
-  g.lo = g.hi = g.tile0 = g.tiles = 0;
-  g.pmin = g.pmax = -1;
-  if (r0 >= g.n * G) return g;
-  g.pmin = g.base + r0 / G;
-  g.pmax = g.base + min((r0 + rows - 1) / G, g.n - 1);
-  g.lo = a.window_left >= 0 ? max(0, g.pmin - a.window_left) : 0;
-  g.hi = static_cast<int>(min(static_cast<long long>(g.pmax) + 1, static_cast<long long>(a.max_pages) * a.page_size));
-  if (g.hi <= g.lo) return g;
-  g.tile0 = g.lo / kTile;
-  g.tiles = (g.hi + kTile - 1) / kTile - g.tile0;
-  return g;
-}
-
 template <int D, bool MX>
 struct Ring {
   static constexpr int kRow = D * (MX ? 1 : 2);               // bytes of a key or value row
@@ -163,7 +133,7 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
   const int lane = threadIdx.x, g8 = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.KV, rb = blockIdx.y / a.KV, b = blockIdx.z;
   const int r0 = rb * ROWS, row_count = min(ROWS, a.T * G - r0);
-  const Range rg = range_of(a, b, r0, ROWS);
+  const Range rg = range_of(a, b, r0, ROWS, kTile);
   const int split_tiles = a.split_keys / kTile;
   const int t0 = rg.tile0 + split * split_tiles;
   const int count = min(rg.tiles - split * split_tiles, split_tiles);
@@ -562,66 +532,6 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
     }
 }
 
-// One CTA per output row: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). Its warps take the runs in turn. Rows that
-// one run finished are skipped.
-constexpr int kCombineWarps = 4;
-template <int D>
-__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedAttnArgs a, int rows) {
-  __shared__ float sm_o[kCombineWarps][D], sm_l[kCombineWarps], sm_m[kCombineWarps];
-  NC_PDL_PROLOGUE();
-  const int G = a.H / a.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = a.T * G;
-  const int r = static_cast<int>(blockIdx.x % per);
-  const int kvh = static_cast<int>(blockIdx.x / per % a.KV), b = static_cast<int>(blockIdx.x / per / a.KV);
-  const int rb = r / rows;
-  const Range rg = range_of(a, b, rb * rows, rows);
-  const int split_tiles = a.split_keys / kTile;
-  if (rg.tiles <= split_tiles) return;
-  const bool real = r < rg.n * G;   // a row behind the last new token is zero
-  const int n = real ? (rg.tiles + split_tiles - 1) / split_tiles : 0;
-  const int rw = min(rows, per);
-  const long long blocks = static_cast<long long>(a.KV) * ((per + rows - 1) / rows);
-  const long long at = ((static_cast<long long>(b) * blocks + rb * a.KV + kvh) * a.splits) * rw + (r - rb * rows);
-  float mx = -CUDART_INF_F;
-  for (int s = threadIdx.x; s < n; s += kCombineWarps * 32) mx = fmaxf(mx, a.part_ml[(at + static_cast<long long>(s) * rw) * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) sm_m[warp] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) mx = fmaxf(mx, sm_m[w]);
-  constexpr int E = D / 32;
-  float o[E], ls = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll 4
-  for (int s = warp; s < n; s += kCombineWarps) {
-    const long long p = at + static_cast<long long>(s) * rw;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
-    const float w = fast_exp2(ml.x - mx);
-    ls = fmaf(w, ml.y, ls);
-    if constexpr (E == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + p * D + lane * 4);
-      o[0] = fmaf(w, x.x, o[0]), o[1] = fmaf(w, x.y, o[1]), o[2] = fmaf(w, x.z, o[2]), o[3] = fmaf(w, x.w, o[3]);
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(a.part_o + p * D + lane * 2);
-      o[0] = fmaf(w, x.x, o[0]), o[1] = fmaf(w, x.y, o[1]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
-  if (lane == 0) sm_l[warp] = ls;
-  __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  float x = 0.0f, y = 0.0f;
-  ls = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) x += sm_o[w][2 * threadIdx.x], y += sm_o[w][2 * threadIdx.x + 1], ls += sm_l[w];
-  const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-  __nv_bfloat16* dst = a.out + ((static_cast<long long>(b) * a.T + r / G) * a.H + kvh * G + r % G) * D;
-  reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = real ? pack_bf16(x * inv, y * inv) : 0u;
-}
-
 // Rows per CTA: the query rows of a kv head in blocks of 8, 16 or 32.
 int row_tiles(const PagedAttnArgs& a) {
   const int rows = a.T * (a.H / a.KV);
@@ -646,8 +556,7 @@ cudaError_t launch_rows(const PagedAttnArgs& a, cudaStream_t s) {
   cudaError_t e = launch_maybe_pdl(paged_rows_kernel<D, MX, NT, P16>, dim3(a.splits, a.KV * blocks, a.B), dim3(32), R::kBytes, s, a);
   if (e != cudaSuccess || a.splits <= 1) return e;
   // always behind the first kernel's tail (it waits for it before it reads anything)
-  return launch_pdl(true, paged_combine_kernel<D>, dim3(static_cast<unsigned>(static_cast<long long>(a.B) * a.T * a.H)),
-                    dim3(kCombineWarps * 32), 0, s, a, static_cast<int>(ROWS));
+  return launch_combine<D>(a, ROWS, kTile, s);
 }
 template <int D, bool MX>
 cudaError_t launch_shape(const PagedAttnArgs& a, cudaStream_t s) {
@@ -675,8 +584,8 @@ PagedPlan paged_rows_plan(const PagedAttnArgs& a) {
   per = (std::min<long long>(std::max<long long>(per, 64), kMaxRun) + kTile - 1) / kTile * kTile;
   PagedPlan p;
   p.split_keys = static_cast<int>(per);
-  // a range that starts inside a tile touches one tile more
-  p.splits = static_cast<int>(((keys + kTile - 1) / kTile + 1 + per / kTile - 1) / (per / kTile));
+  // a window may start inside a tile and touch one more
+  p.splits = static_cast<int>(((keys + kTile - 1) / kTile + (a.window_left >= 0 ? 1 : 0) + per / kTile - 1) / (per / kTile));
   if (p.splits > 1) {
     const long long rw = std::min<long long>(rows, static_cast<long long>(a.T) * G);
     p.part_o = units * p.splits * rw * a.D;

@@ -48,13 +48,17 @@ struct PagedAttnArgs {
   int* status = nullptr;
 };
 
-// Work split of the few-rows kernel: keys per CTA and the floats of workspace it needs (0: none).
+// Work split: keys per run and the floats of workspace it needs (0: none).
 struct PagedPlan {
   int splits = 1, split_keys = 0;
   long long part_o = 0, part_ml = 0;
 };
 PagedPlan paged_rows_plan(const PagedAttnArgs& a);
 const char* paged_rows_attention(const PagedAttnArgs& a, cudaStream_t s);
+// The same for many rows per kv head (`paged_chunk_takes`: sizes it is meant for and can do).
+bool paged_chunk_takes(const PagedAttnArgs& a);
+PagedPlan paged_chunk_plan(const PagedAttnArgs& a);
+const char* paged_chunk_attention(const PagedAttnArgs& a, cudaStream_t s);
 
 struct SampleArgs {
   const void* logits = nullptr;  // bf16 or fp32 rows, leading dimension ld

@@ -144,14 +144,16 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   a.scale = static_cast<float>(scale);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.status = ncbind::device_status(k_pool.get_device());
-  const nc::PagedPlan p = nc::paged_rows_plan(a);
+  const bool chunk = nc::paged_chunk_takes(a);
+  const nc::PagedPlan p = chunk ? nc::paged_chunk_plan(a) : nc::paged_rows_plan(a);
   a.splits = p.splits, a.split_keys = p.split_keys;
   Tensor work;
   if (p.splits > 1) {   // a buffer of its own per call: calls on other streams or in other graphs never share it
     work = torch::empty({p.part_o + p.part_ml}, q.options().dtype(torch::kFloat32));
     a.part_o = work.data_ptr<float>(), a.part_ml = a.part_o + p.part_o;
   }
-  const char* err = nc::paged_rows_attention(a, at::cuda::getCurrentCUDAStream());
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  const char* err = chunk ? nc::paged_chunk_attention(a, stream) : nc::paged_rows_attention(a, stream);
   TORCH_CHECK(err == nullptr, err);
   return out;
 }
