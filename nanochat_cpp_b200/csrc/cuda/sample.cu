@@ -8,16 +8,21 @@
 // the gap between neighbouring tokens. p itself is computed in 64-bit floating point; a logit more than 33 t below the
 // maximum has no mass and is never looked at again.
 //
-// One CTA per row. A histogram over z (bins of equal width below the maximum: monotone in z, and spread, where the
-// bits of z would put most logits into a handful of bins) finds a cut below which nothing can be kept. If at most 1024
-// logits lie above it - the usual settings - they are collected in shared memory, sorted, and everything else happens there: only these
-// need the exponential. Otherwise the thresholds are narrowed down by further histograms over the bits of z, and the
-// draw walks the vocabulary by halving it among the warps.
+// A row belongs to a cluster of 1, 2, 4 or 8 CTAs (more where there are few rows); each copies its slice into shared
+// memory, so the logits are read from memory once. A histogram over z (bins of equal width below the maximum: monotone in z, and
+// spread, where the bits of z would put most logits into a handful of bins) finds a cut below which nothing can be kept. If at
+// most 1024 logits lie above it - the usual settings - they are collected in the first CTA, sorted, and
+// everything else happens there: only these need the exponential. Otherwise the thresholds are narrowed down by
+// further histograms over the bits of z, and the draw walks the vocabulary by halving it among the warps. Bound by the
+// chain of such steps (each a pass over the slice and a cluster barrier) for few rows, by 64-bit arithmetic for many.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "ptx.cuh"
 #include "serving.h"
 
 namespace nc {
@@ -26,10 +31,12 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kPerThread = kBins / kThreads;
 constexpr int kList = 1024;      // candidates that are sorted in shared memory
+constexpr int kMaxCluster = 8;
 constexpr float kReach = 33.0f;  // e^-33 < 2^-47: no mass beyond
 
 // z as a number that orders like its bits: NaN becomes -infinity, -0 becomes 0.
@@ -42,15 +49,27 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+// This CTA's slice of the row: elements [0, n) stand for indices `first` + i. `p` is in shared or global memory.
 template <class T>
-struct RowView {
+struct Slice {
   const T* p;
-  int n;
+  int n, first;
   __device__ __forceinline__ float at(int i) const {
     if constexpr (sizeof(T) == 2) return clean(__bfloat162float(p[i]));
     else return clean(p[i]);
   }
-  // f(index, z) for every element, by 16-byte loads between the first and the last aligned address
+  template <class F>
+  __device__ __forceinline__ static void spread(const uint4& w, int i, F f) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(16 / sizeof(T)); ++e) {
+      float z;
+      if constexpr (sizeof(T) == 2) z = __uint_as_float((e & 1) ? (u[e / 2] & 0xffff0000u) : (u[e / 2] << 16));
+      else z = __uint_as_float(u[e]);
+      f(i + e, clean(z));
+    }
+  }
+  // f(i, z) for every element, by 16-byte loads between the first and the last aligned address
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     constexpr int E = 16 / sizeof(T);
@@ -58,64 +77,98 @@ struct RowView {
     const int vecs = (n - head) / E;
     if (threadIdx.x < head) f(static_cast<int>(threadIdx.x), at(threadIdx.x));
 #pragma unroll 2
-    for (int v = threadIdx.x; v < vecs; v += kThreads) {
-      const int i = head + v * E;
-      const uint4 w = *reinterpret_cast<const uint4*>(p + i);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float z;
-        if constexpr (sizeof(T) == 2) z = __uint_as_float((e & 1) ? (u[e / 2] & 0xffff0000u) : (u[e / 2] << 16));
-        else z = __uint_as_float(u[e]);
-        f(i + e, clean(z));
-      }
-    }
+    for (int v = threadIdx.x; v < vecs; v += kThreads)
+      spread(*reinterpret_cast<const uint4*>(p + head + v * E), head + v * E, f);
     for (int i = head + vecs * E + threadIdx.x; i < n; i += kThreads) f(i, at(i));
   }
 };
 
-// exp((z - zmax) / t) in 64 bits by argument reduction to |r| <= ln2 / 64 with a table of 2^(j/32) and the Taylor
-// polynomial to the fifth power (remainder below 2^-47 of the value).
+// Mass of a logit: exp((z - zmax) / t) in 64 bits, as an integer in units of 2^-fraction. With y = (z - zmax) / t * 32 / ln 2
+// split into a whole number k and r in [-1/2, 1/2], p = 2^(k / 32) * 2^(r / 32): the first from a table of 32 and the
+// exponent field, the second by its Taylor polynomial to the fourth power (remainder below 2^-39 of p).
 struct Exponent {
-  double zmax, inv_t;
+  double zmax, per;      // per = 32 / (ln 2 * t)
   const double* table;   // shared: 2^(j / 32)
-  int fraction;          // bits behind the point of a mass
-  float z_cut;           // below: no mass
-  __device__ __forceinline__ double p(float z) const {
-    const double x = (static_cast<double>(z) - zmax) * inv_t;
-    constexpr double kPerLn2 = 46.16624130844682838;   // 32 / ln 2
-    constexpr double kLn2Hi = 0x1.62e42fefa0000p-6, kLn2Lo = 0x1.cf79abc9e3b3ap-45;   // ln 2 / 32 in two parts
-    const double kd = rint(x * kPerLn2);
-    const int k = static_cast<int>(kd);
-    const double r = fma(kd, -kLn2Lo, fma(kd, -kLn2Hi, x));
-    const double q = r * fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0);
+  float z_max, z_cut;    // z_cut: below there is no mass
+  int fraction;
+  __device__ __forceinline__ double scaled(float z) const {   // p * 2^fraction, z_cut <= z
+    constexpr double kShift = 6755399441055744.0;              // 1.5 * 2^52: adding it leaves the whole number in the low bits
+    constexpr double kLn = 0.021660849392498290;               // ln 2 / 32
+    const double d = static_cast<double>(z) - zmax;
+    const double kd = fma(d, per, kShift);
+    const int k = __double2loint(kd);
+    const double r = fma(d, per, -(kd - kShift));
+    const double q = fma(r, fma(r, fma(r, fma(r, kLn * kLn * kLn * kLn / 24, kLn * kLn * kLn / 6), kLn * kLn / 2), kLn), 1.0);
     const double s = table[k & 31];
-    return ldexp(fma(s, q, s), k >> 5);
+    return q * __hiloint2double(__double2hiint(s) + (((k >> 5) + fraction) << 20), __double2loint(s));
   }
-  __device__ __forceinline__ u64 mass_of(double p) const {   // round(p 2^fraction), p <= 1
-    return static_cast<u64>(__double2ll_rn(p * static_cast<double>(1ull << fraction)));
+  __device__ __forceinline__ static u64 whole(double m) {     // round(m), 0 <= m < 2^51
+    return static_cast<u64>(__double_as_longlong(m + 4503599627370496.0)) & 0xfffffffffffffull;
   }
-  __device__ __forceinline__ u64 mass(float z) const { return z < z_cut ? 0ull : z == static_cast<float>(zmax) ? 1ull << fraction : mass_of(p(z)); }
+  __device__ __forceinline__ u64 one() const { return 1ull << fraction; }
+  __device__ __forceinline__ u64 mass(float z) const { return z < z_cut ? 0ull : z == z_max ? one() : whole(scaled(z)); }
 };
 
 struct Shared {
   double table[32];
-  u64 list[kList];             // sorted candidates: order key in the high half, ~index in the low
-  u64 list_mass[kList];
   union {
-    unsigned count[kBins];
-    u64 mass[kBins];
+    u64 hist[kBins];           // masses or counts of this CTA, summed over the cluster by whoever reads them
+    unsigned limb[3][kBins];   // masses in three parts of 16 bits (32-bit additions are native, 64-bit ones a loop)
+    struct {                   // the short way, in the first CTA
+      u64 sorted[kList], list_mass[kList], bucket[kThreads];
+    };
   };
+  u64 list[kList];             // candidates: order key in the high half, ~index in the low
+  unsigned count[kBins];
+  unsigned cursor[kBins];      // the first CTA: where the next candidate of a bin goes; in the end where its last one ends
   u64 warp_sum[kWarps];
+  u64 sums[2];                 // this CTA's totals, read by the others (two, used in turn)
   float warp_max[kWarps], warp_min[kWarps];
   int warp_arg[kWarps];
+  float top, bottom;           // of this CTA's slice
+  int arg;
   unsigned n;                  // candidates collected
   int bin;
   u64 below, inside;
   int lo, hi;
   u64 target;
-  int answer;
+  int answer;                  // index of a found element, or -1: written by the CTA that has it, into every CTA
+  uint32_t cut_key;            // threshold found by the first CTA, written into every CTA
+  int cut_last;                // kNoList: too many candidates for the list
 };
+constexpr int kNoList = -2;
+
+// What a CTA knows of its cluster, and the steps that need all of it.
+struct Cluster {
+  int size, rank, turn;
+  __device__ __forceinline__ void sync() const {
+    if (size > 1) cluster_sync_all();
+    else __syncthreads();
+  }
+  template <class X>
+  __device__ __forceinline__ uint32_t peer(const X* x, int r) const { return mapa_u32(x, r); }
+};
+__device__ __forceinline__ u64 ld_peer_u64(uint32_t at) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_peer_u32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_peer_u64(uint32_t at, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ void st_peer_u32(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t add_peer_u32(uint32_t at, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
+  return old;
+}
 
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {   // inclusive
 #pragma unroll
@@ -137,69 +190,132 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& sm, u64& total) {
   __syncthreads();
   if (lane == 31) sm.warp_sum[warp] = v;
   __syncthreads();
-  const u64 w = warp_scan(sm.warp_sum[lane], lane);
+  const u64 w = warp_scan(lane < kWarps ? sm.warp_sum[lane] : 0, lane);
   total = __shfl_sync(0xffffffffu, w, 31);
   const u64 before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
   return v + (warp > 0 ? before : 0);
 }
 
-// Sorts n2 (a power of two) 64-bit values in shared memory, ascending or descending.
-__device__ void sort_list(u64* v, int n2, bool descending) {
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n2 / 2; t += kThreads) {
-        const int i = 2 * j * (t / j) + t % j, o = i + j;
-        const u64 x = v[i], y = v[o];
-        const bool up = ((i & k) == 0) != descending;
-        if ((x > y) == up) v[i] = y, v[o] = x;
-      }
-    }
+// The sum of one value per thread over the cluster; `before` is the part of CTAs of lower rank, `mine` this CTA's.
+__device__ __forceinline__ u64 cluster_sum(u64 v, Shared& sm, Cluster& cl, u64& before, u64& mine) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_total(v);
   __syncthreads();
+  if (lane == 0) sm.warp_sum[warp] = v;
+  __syncthreads();
+  mine = warp_total(lane < kWarps ? sm.warp_sum[lane] : 0);
+  before = 0;
+  if (cl.size == 1) return mine;
+  cl.turn ^= 1;   // the slot of the turn before may still be read
+  if (threadIdx.x == 0) sm.sums[cl.turn] = mine;
+  cl.sync();
+  u64 all = 0;
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r)
+    if (r < cl.size) {
+      const u64 x = ld_peer_u64(cl.peer(&sm.sums[cl.turn], r));
+      if (r < cl.rank) before += x;
+      all += x;
+    }
+  return all;
 }
 
-// The first index at which the running weight (vocabulary order) exceeds `target`; w(i) is the weight of element i.
-// The range is divided among the warps until one warp can walk it. `total` must exceed target.
-template <class W>
-__device__ int order_search(Shared& sm, int n, u64 target, W w) {
+// f(rank) for every CTA of the cluster, unrolled so that the reads of all of them are in flight together
+template <class F>
+__device__ __forceinline__ void each_peer(const Cluster& cl, F f) {
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r)
+    if (r < cl.size) f(r);
+}
+
+// The bins of all CTAs, kPerThread neighbouring ones per thread.
+__device__ __forceinline__ void cluster_bins(Shared& sm, const Cluster& cl, u64 (&x)[kPerThread]) {
+  cl.sync();
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) x[i] = 0;
+  each_peer(cl, [&](int r) {
+    const uint32_t at = cl.peer(&sm.hist[kPerThread * threadIdx.x], r);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) x[i] += ld_peer_u64(at + 8 * i);
+  });
+}
+__device__ __forceinline__ void cluster_counts(Shared& sm, const Cluster& cl, const unsigned* bins, u64 (&x)[kPerThread]) {
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) x[i] = 0;
+  each_peer(cl, [&](int r) {
+    const uint32_t at = cl.peer(&bins[kPerThread * threadIdx.x], r);
+#pragma unroll
+    for (int i = 0; i < kPerThread; i += 2) {
+      const u64 two = ld_peer_u64(at + 4 * i);
+      x[i] += two & 0xffffffffu, x[i + 1] += two >> 32;
+    }
+  });
+}
+
+// The first index at which the running weight (vocabulary order) exceeds target_of(total weight), or -1; w(i, z) is the
+// weight of element i of the slice. The CTA that holds it divides its slice among its warps until one warp can walk it.
+template <class T, class Target, class W>
+__device__ int order_search(Shared& sm, Cluster& cl, const Slice<T>& row, Target target_of, W w) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int lo = 0, hi = n;
-  while (hi - lo > 64) {
-    const int seg = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
-    const int a = min(lo + warp * seg, hi), b = min(a + seg, hi);
-    u64 s = 0;
-    for (int i = a + lane; i < b; i += 32) s += w(i);
-    s = warp_total(s);
-    __syncthreads();
-    if (lane == 0) sm.warp_sum[warp] = s;
-    __syncthreads();
+  u64 s = 0, before, mine;
+  // the first division is by slices of the CTAs and, inside, by sixteenths for its warps
+  int lo = 0, hi = row.n;
+  int seg = ((row.n + kWarps - 1) / kWarps + 31) / 32 * 32;
+  {
+    const int a = min(warp * seg, hi), b = min(a + seg, hi);
+#pragma unroll 4
+    for (int i = a + lane; i < b; i += 32) s += w(i, row.at(i));
+  }
+  u64 target = target_of(cluster_sum(s, sm, cl, before, mine));
+  const bool here = target >= before && target - before < mine;
+  if (threadIdx.x == 0) sm.answer = -1;
+  cl.sync();
+  if (here) {
+    target -= before;
+    for (bool summed = true; hi - lo > 64; summed = false) {
+      if (!summed) {
+        seg = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+        const int a = min(lo + warp * seg, hi), b = min(a + seg, hi);
+        u64 t = 0;
+        for (int i = a + lane; i < b; i += 32) t += w(i, row.at(i));
+        t = warp_total(t);
+        __syncthreads();
+        if (lane == 0) sm.warp_sum[warp] = t;
+        __syncthreads();
+      }
+      if (warp == 0) {
+        const u64 x = lane < kWarps ? sm.warp_sum[lane] : 0, c = warp_scan(x, lane);
+        const unsigned over = __ballot_sync(0xffffffffu, c > target);
+        const int f = over ? __ffs(over) - 1 : kWarps - 1;
+        if (lane == f) {
+          sm.lo = min(lo + f * seg, hi), sm.hi = min(lo + (f + 1) * seg, hi);
+          sm.target = target - (c - x);
+        }
+      }
+      __syncthreads();
+      lo = sm.lo, hi = sm.hi, target = sm.target;
+      __syncthreads();
+    }
     if (warp == 0) {
-      const u64 c = warp_scan(sm.warp_sum[lane], lane);
-      const unsigned over = __ballot_sync(0xffffffffu, c > target);
-      const int f = over ? __ffs(over) - 1 : kWarps - 1;
-      if (lane == f) {
-        sm.lo = min(lo + f * seg, hi), sm.hi = min(lo + (f + 1) * seg, hi);
-        sm.target = target - (c - sm.warp_sum[lane]);
+      int found = -1;
+      u64 run = 0;
+      for (int i0 = lo; i0 < hi && found < 0; i0 += 32) {
+        const u64 x = i0 + lane < hi ? w(i0 + lane, row.at(i0 + lane)) : 0;
+        const u64 c = warp_scan(x, lane) + run;
+        const unsigned over = __ballot_sync(0xffffffffu, c > target);
+        if (over) found = i0 + __ffs(over) - 1;
+        run = __shfl_sync(0xffffffffu, c, 31);
+      }
+      if (lane < cl.size) {
+        const int index = found < 0 ? -1 : row.first + found;
+        if (cl.size == 1) sm.answer = index;
+        else st_peer_u32(cl.peer(&sm.answer, lane), static_cast<uint32_t>(index));
       }
     }
-    __syncthreads();
-    lo = sm.lo, hi = sm.hi, target = sm.target;
   }
-  if (warp == 0) {
-    int found = -1;
-    u64 run = 0;
-    for (int i0 = lo; i0 < hi && found < 0; i0 += 32) {
-      const u64 x = i0 + lane < hi ? w(i0 + lane) : 0;
-      const u64 c = warp_scan(x, lane) + run;
-      const unsigned over = __ballot_sync(0xffffffffu, c > target);
-      if (over) found = i0 + __ffs(over) - 1;
-      run = __shfl_sync(0xffffffffu, c, 31);
-    }
-    if (lane == 0) sm.answer = found;
-  }
-  __syncthreads();
+  cl.sync();
   const int r = sm.answer;
-  __syncthreads();
+  cl.sync();
   return r;
 }
 
@@ -210,43 +326,72 @@ struct Threshold {
   __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
 };
 
-// Descending histogram search over the keys of the elements that `in` selects, all within [lo, hi]: the largest key at
-// which the running weight (from the top) reaches `want` > 0. On return sm.below is the weight strictly above that key.
-template <class T, class In, class W>
-__device__ uint32_t key_search(Shared& sm, const RowView<T>& row, uint32_t lo, uint32_t hi, double want, u64 above, In in, W w) {
-  while (lo < hi) {
+// x: bins of the whole row, from the top. Finds the first bin at which the running weight reaches want_of(total): sm.bin is
+// its number (-1: none) and sm.below the weight before it. Returns the running weight before the thread's bins.
+template <class Want>
+__device__ __forceinline__ u64 first_reaching(Shared& sm, const u64 (&x)[kPerThread], u64 above, Want want_of, u64& total) {
+  u64 sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) sum += x[i];
+  if (threadIdx.x == 0) sm.bin = -1;
+  const u64 start = block_scan(sum, sm, total) + above - sum;
+  const double want = want_of(total);
+  u64 c = start;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    if (static_cast<double>(c) < want && static_cast<double>(c + x[i]) >= want) sm.bin = kPerThread * threadIdx.x + i, sm.below = c;
+    c += x[i];
+  }
+  __syncthreads();
+  return start;
+}
+
+// Descending search among the elements that `in` selects: the largest key at which the running weight (from the top) reaches
+// `want` > 0. First over the bins of z, then over the bits of the keys inside the bin. On return sm.below is the
+// weight strictly above that key.
+template <class T, class Bin, class In, class W>
+__device__ uint32_t key_search(Shared& sm, Cluster& cl, const Slice<T>& row, const Exponent& ex, Bin bin_of, float per, double want, In in, W w) {
+  uint32_t lo = order_key(ex.z_cut), hi = order_key(ex.z_max);
+  u64 above = 0, total, x[kPerThread];
+  int bin = -1;
+  for (bool first = true; first || lo < hi; first = false) {
     int shift = 0;
     while (((hi - lo) >> shift) >= kBins) ++shift;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sm.mass[i] = 0;
+    cl.sync();   // the bins of the step before have been read by all
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
     __syncthreads();
     row.each([&](int i, float z) {
+      if (z < ex.z_cut) return;
       const uint32_t k = order_key(z);
-      if (k >= lo && k <= hi && in(i, z, k)) atomicAdd(&sm.mass[(hi - k) >> shift], w(z));
+      if (first) {
+        if (in(i, z, k)) atomicAdd(&sm.hist[bin_of(z)], w(z));
+      } else if (k >= lo && k <= hi && bin_of(z) == bin && in(i, z, k)) {
+        atomicAdd(&sm.hist[(hi - k) >> shift], w(z));
+      }
     });
+    cluster_bins(sm, cl, x);
+    first_reaching(sm, x, above, [&](u64) { return want; }, total);
+    const int j = sm.bin;
+    const u64 before_j = sm.below;
     __syncthreads();
-    // two neighbouring bins per thread
-    u64 total;
-    const u64 x0 = sm.mass[2 * threadIdx.x], x1 = sm.mass[2 * threadIdx.x + 1];
-    const u64 c1 = block_scan(x0 + x1, sm, total) + above, c0 = c1 - x1, before = c0 - x0;
-    if (threadIdx.x == 0) sm.bin = -1;
-    __syncthreads();
-    const bool r0 = static_cast<double>(c0) >= want, rb = static_cast<double>(before) >= want, r1 = static_cast<double>(c1) >= want;
-    if (r0 && !rb) sm.bin = 2 * threadIdx.x, sm.below = before;
-    else if (r1 && !r0) sm.bin = 2 * threadIdx.x + 1, sm.below = c0;
-    __syncthreads();
-    int j = sm.bin;
-    if (j < 0) {   // rounding of `want` past the total: the last key
-      j = static_cast<int>((hi - lo) >> shift);
-      if (threadIdx.x == 0) sm.below = above + total - sm.mass[j];
+    if (j >= 0) above = before_j;
+    if (j < 0) {      // rounding of `want` past the total: everything is kept
+      if (threadIdx.x == 0) sm.below = above + total;
       __syncthreads();
+      return lo;
     }
-    above = sm.below;
-    const uint32_t new_hi = hi - (static_cast<uint32_t>(j) << shift);
-    const u64 span = (1ull << shift) - 1;
-    lo = static_cast<u64>(new_hi) - lo > span ? static_cast<uint32_t>(new_hi - span) : lo;
-    hi = new_hi;
-    __syncthreads();
+    if (first) {
+      // the keys that the bin can hold: a hundredth of a bin more on either side, far above the rounding of bin_of
+      bin = j;
+      const float z_lo = ex.z_max - (j + 1.01f) / per, z_hi = ex.z_max - (j - 0.01f) / per;
+      if (per < 1e30f && z_lo > ex.z_cut && j < kBins - 1) lo = order_key(z_lo);
+      if (per < 1e30f && z_hi < ex.z_max) hi = order_key(z_hi);
+    } else {
+      const uint32_t new_hi = hi - (static_cast<uint32_t>(j) << shift);
+      const u64 span = (1ull << shift) - 1;
+      lo = static_cast<u64>(new_hi) - lo > span ? static_cast<uint32_t>(new_hi - span) : lo;
+      hi = new_hi;
+    }
   }
   if (threadIdx.x == 0) sm.below = above;
   __syncthreads();
@@ -254,186 +399,383 @@ __device__ uint32_t key_search(Shared& sm, const RowView<T>& row, uint32_t lo, u
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 1) sample_rows_kernel(const SampleArgs a) {
-  __shared__ Shared sm;
-  const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const RowView<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleArgs a, int cluster, int slice, int staged) {
+  extern __shared__ __align__(16) uint8_t dyn[];
+  Shared& sm = *reinterpret_cast<Shared*>(dyn);
+  Cluster cl;
+  cl.size = cluster, cl.rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0, cl.turn = 0;
+  const int r = blockIdx.x / cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Slice<T> row;
+  row.first = min(cl.rank * slice, a.vocab);
+  row.n = min(slice, a.vocab - row.first);
+  const Slice<T> global{static_cast<const T*>(a.logits) + r * a.ld + row.first, row.n, row.first};
   const float t = a.temperature_rows != nullptr ? a.temperature_rows[r] : a.temperature;
   const float top_p = a.top_p_rows != nullptr ? a.top_p_rows[r] : a.top_p;
   const float min_p = a.min_p_rows != nullptr ? a.min_p_rows[r] : a.min_p;
   int k = a.top_k_rows != nullptr ? a.top_k_rows[r] : a.top_k;
   if (k <= 0 || k > a.vocab) k = a.vocab;
-  if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
 
-  // ---- the largest logit (lowest index of equals) and the smallest above -infinity
+  // ---- the largest logit (lowest index of equals) and the smallest above -infinity; the slice goes to shared memory
+  // with the alignment that it has, so that 16-byte pieces stay 16-byte pieces
+  T* stage = reinterpret_cast<T*>(dyn + (sizeof(Shared) + 15) / 16 * 16) + (reinterpret_cast<uintptr_t>(global.p) & 15) / sizeof(T);
+  row.p = staged ? stage : global.p;
   float zmax = -CUDART_INF_F, zmin = CUDART_INF_F;
   int arg = 0x7fffffff;
-  row.each([&](int i, float z) {
-    if (z > zmax || (z == zmax && i < arg)) zmax = z, arg = i;
-    if (z > -CUDART_INF_F) zmin = fminf(zmin, z);
-  });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float oz = __shfl_xor_sync(0xffffffffu, zmax, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, arg, o);
-    if (oz > zmax || (oz == zmax && oi < arg)) zmax = oz, arg = oi;
-    zmin = fminf(zmin, __shfl_xor_sync(0xffffffffu, zmin, o));
+  {
+    constexpr int E = 16 / sizeof(T);
+    const int head = min(row.n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(global.p) & 15)) & 15) / sizeof(T)));
+    const int vecs = (row.n - head) / E;
+    auto see = [&](int i, float z) {
+      if (z > zmax || (z == zmax && i < arg)) zmax = z, arg = i;
+      if (z > -CUDART_INF_F) zmin = fminf(zmin, z);
+    };
+    if (threadIdx.x < head) {
+      if (staged) stage[threadIdx.x] = global.p[threadIdx.x];
+      see(threadIdx.x, global.at(threadIdx.x));
+    }
+#pragma unroll 4
+    for (int v = threadIdx.x; v < vecs; v += kThreads) {
+      const uint4 x = __ldcs(reinterpret_cast<const uint4*>(global.p + head + v * E));
+      if (staged) *reinterpret_cast<uint4*>(stage + head + v * E) = x;
+      Slice<T>::spread(x, head + v * E, see);
+    }
+    for (int i = head + vecs * E + threadIdx.x; i < row.n; i += kThreads) {
+      if (staged) stage[i] = global.p[i];
+      see(i, global.at(i));
+    }
   }
-  if (lane == 0) sm.warp_max[warp] = zmax, sm.warp_arg[warp] = arg, sm.warp_min[warp] = zmin;
-  __syncthreads();
-  zmax = sm.warp_max[lane], arg = sm.warp_arg[lane], zmin = sm.warp_min[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float oz = __shfl_xor_sync(0xffffffffu, zmax, o);
-    const int oi = __shfl_xor_sync(0xffffffffu, arg, o);
+  if (arg != 0x7fffffff) arg += row.first;
+  auto take = [&](float oz, int oi, float om) {
     if (oz > zmax || (oz == zmax && oi < arg)) zmax = oz, arg = oi;
-    zmin = fminf(zmin, __shfl_xor_sync(0xffffffffu, zmin, o));
+    zmin = fminf(zmin, om);
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    take(__shfl_xor_sync(0xffffffffu, zmax, o), __shfl_xor_sync(0xffffffffu, arg, o), __shfl_xor_sync(0xffffffffu, zmin, o));
+  if (lane == 0) sm.warp_max[warp] = zmax, sm.warp_arg[warp] = arg, sm.warp_min[warp] = zmin;
+  if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sm.count[i] = 0;
+  if (threadIdx.x == 0) sm.n = 0;
+  __syncthreads();
+  zmax = sm.warp_max[lane % kWarps], arg = sm.warp_arg[lane % kWarps], zmin = sm.warp_min[lane % kWarps];
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+    take(__shfl_xor_sync(0xffffffffu, zmax, o), __shfl_xor_sync(0xffffffffu, arg, o), __shfl_xor_sync(0xffffffffu, zmin, o));
+  if (cl.size > 1) {
+    if (threadIdx.x == 0) sm.top = zmax, sm.arg = arg, sm.bottom = zmin;
+    cl.sync();
+    each_peer(cl, [&](int c) {
+      take(__uint_as_float(ld_peer_u32(cl.peer(&sm.top, c))), static_cast<int>(ld_peer_u32(cl.peer(&sm.arg, c))),
+           __uint_as_float(ld_peer_u32(cl.peer(&sm.bottom, c))));
+    });
   }
   if (zmax == -CUDART_INF_F || !(t > 0.0f) || k == 1 || !(top_p > 0.0f) || !(min_p <= 1.0f)) {
-    if (threadIdx.x == 0) a.out[r] = zmax == -CUDART_INF_F ? -1 : arg;
+    if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = zmax == -CUDART_INF_F ? -1 : arg;
+    if (cl.size > 1) cl.sync();   // no CTA leaves while another reads its shared memory
     return;
   }
   Exponent ex;
-  ex.zmax = static_cast<double>(zmax), ex.inv_t = 1.0 / static_cast<double>(t), ex.table = sm.table;
+  ex.zmax = static_cast<double>(zmax), ex.z_max = zmax, ex.table = sm.table;
+  ex.per = 46.166241308446828384 / static_cast<double>(t);
   int log_v = 0;
   while ((1ll << log_v) < a.vocab) ++log_v;
   ex.fraction = min(46, 62 - log_v);
   ex.z_cut = fmaxf(zmax - kReach * t, -3.402823466e38f);   // -infinity has no mass at any temperature
-  const double u = fmax(static_cast<double>(a.u[r]), 0.0), pmin = static_cast<double>(min_p), want_p = static_cast<double>(top_p);
+  const double u = fmax(static_cast<double>(a.u[r]), 0.0), want_p = static_cast<double>(top_p);
+  const double pmin = static_cast<double>(min_p) * static_cast<double>(ex.one());   // in units of mass
   const bool nucleus = top_p < 1.0f, filtered = k < a.vocab || nucleus || min_p > 0.0f;
-  const uint32_t max_key = order_key(zmax);
 
   Threshold cut;                    // what top-k and top-p keep, when the long way is taken
-  cut.key = order_key(ex.z_cut), cut.last = 0x7fffffff;
+  cut.key = order_key(ex.z_cut);
   if (filtered) {
     const float width = fminf(zmax - zmin, kReach * t);
     const float per = width > 0.0f ? static_cast<float>(kBins) / width : 0.0f;
     auto bin_of = [&](float z) { return z == zmax ? 0 : min(static_cast<int>((zmax - z) * per), kBins - 1); };
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sm.count[i] = 0;
-    if (threadIdx.x == 0) sm.bin = kBins - 1, sm.n = 0;
-    __syncthreads();
     row.each([&](int, float z) {
       if (z >= ex.z_cut) atomicAdd(&sm.count[bin_of(z)], 1u);
     });
-    __syncthreads();
+    cl.sync();
+    u64 x[kPerThread], total;
+    cluster_counts(sm, cl, sm.count, x);
     // the first bin at which k logits are reached, and the last one that min_p can keep anything of
-    u64 total;
-    const unsigned n0 = sm.count[2 * threadIdx.x], n1 = sm.count[2 * threadIdx.x + 1];
-    const u64 c1 = block_scan(n0 + n1, sm, total), c0 = c1 - n1, before = c0 - n0;
-    if (c0 >= static_cast<u64>(k) && before < static_cast<u64>(k)) sm.bin = 2 * threadIdx.x;
-    else if (c1 >= static_cast<u64>(k) && c0 < static_cast<u64>(k)) sm.bin = 2 * threadIdx.x + 1;
-    __syncthreads();
-    const int bin_k = sm.bin;
+    const u64 start = first_reaching(sm, x, 0, [&](u64) { return static_cast<double>(k); }, total);
+    const int bin_k = sm.bin < 0 ? kBins - 1 : sm.bin;
+    const u64 above_k = sm.bin < 0 ? 0 : sm.below;
     int bin_m = kBins - 1;
     if (min_p > 0.0f) {   // rounded down generously; the exact comparison follows
       const float z = zmax + t * logf(min_p) * 1.0001f - 1e-5f * (fabsf(zmax) + 1.0f);
       bin_m = z > ex.z_cut ? bin_of(z) : kBins - 1;
     }
     const int bin_cut = min(bin_k, bin_m);
-    __syncthreads();
-    if (bin_cut / 2 == static_cast<int>(threadIdx.x)) sm.inside = bin_cut & 1 ? c1 : c0;
-    if (bin_k / 2 == static_cast<int>(threadIdx.x)) sm.below = bin_k & 1 ? c0 : before;
-    __syncthreads();
-    const u64 n_cut = sm.inside, above_k = sm.below;
+    u64 c = start;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      sm.cursor[kPerThread * threadIdx.x + i] = static_cast<unsigned>(c);
+      c += x[i];
+      if (static_cast<int>(kPerThread * threadIdx.x) + i == bin_cut) sm.inside = c;
+    }
+    cl.sync();
+    const u64 n_cut = sm.inside;
 
     if (n_cut <= kList) {
-      // ---- the short way: collect, sort, decide
+      // ---- the short way, in the first CTA: candidates go to their bin's places, are ranked inside it, and decided on
       row.each([&](int i, float z) {
-        if (z >= ex.z_cut && bin_of(z) <= bin_cut)
-          sm.list[atomicAdd(&sm.n, 1u)] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~i);
+        if (z < ex.z_cut) return;
+        const int bin = bin_of(z);
+        if (bin > bin_cut) return;
+        const u64 e = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
+        if (cl.size == 1) sm.list[atomicAdd(&sm.cursor[bin], 1u)] = e;
+        else st_peer_u64(cl.peer(sm.list, 0) + add_peer_u32(cl.peer(&sm.cursor[bin], 0), 1u) * 8, e);
       });
-      __syncthreads();
-      const int n = static_cast<int>(sm.n);
-      int n2 = 2;
-      while (n2 < n) n2 <<= 1;
-      for (int i = n + threadIdx.x; i < n2; i += kThreads) sm.list[i] = 0;
-      sort_list(sm.list, n2, true);
-      const int i = threadIdx.x;
-      u64 mine = 0, total_k;
-      if (i < n && i < k) {
-        const float z = key_value(static_cast<uint32_t>(sm.list[i] >> 32));
-        const double p = z == zmax ? 1.0 : ex.p(z);
-        if (i == 0 || p >= pmin) mine = ex.mass_of(p);
+      cl.sync();
+      if (cl.rank != 0) return;   // nobody reads this CTA's memory any more
+      const int n = static_cast<int>(n_cut);
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 e = sm.list[i];
+        const int bin = bin_of(key_value(static_cast<uint32_t>(e >> 32)));
+        const int from = bin > 0 ? sm.cursor[bin - 1] : 0, to = sm.cursor[bin];
+        int rank = from;
+        for (int j = from; j < to; ++j) rank += sm.list[j] > e;
+        sm.sorted[rank] = e;
       }
-      const u64 incl = block_scan(mine, sm, total_k);
-      bool keep = i < n && i < k && mine > 0;
-      if (nucleus && i > 0) keep = keep && static_cast<double>(incl - mine) < want_p * static_cast<double>(total_k);
-      // Back to vocabulary order: index in the high half, place in the list in the low; what is not kept goes last.
-      sm.list_mass[i] = keep ? mine : 0;
-      const uint32_t index = i < n ? ~static_cast<uint32_t>(sm.list[i]) : 0xffffffffu;
+      sm.bucket[threadIdx.x] = 0;
       __syncthreads();
-      if (i < n2) sm.list[i] = (static_cast<u64>(keep ? index : 0xffffffffu) << 32) | static_cast<uint32_t>(i);
-      sort_list(sm.list, n2, false);
-      u64 w = i < n2 && (sm.list[i] >> 32) != 0xffffffffu ? sm.list_mass[static_cast<uint32_t>(sm.list[i])] : 0;
+      // two neighbours per thread
+      constexpr int N = kList / kThreads;
+      u64 mine[N], sum = 0, total_k;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int i = N * threadIdx.x + e;
+        mine[e] = 0;
+        if (i < n && i < k) {
+          const float z = key_value(static_cast<uint32_t>(sm.sorted[i] >> 32));
+          const double p = z == zmax ? static_cast<double>(ex.one()) : ex.scaled(z);
+          if (i == 0 || p >= pmin) mine[e] = Exponent::whole(p);
+        }
+        sum += mine[e];
+      }
+      u64 before = block_scan(sum, sm, total_k) - sum;
+      // Back to vocabulary order: the mass of each of kThreads ranges of indices, the range in which the draw falls,
+      // and the few candidates inside it.
+      const unsigned range = (a.vocab + kThreads - 1) / kThreads;
+      uint32_t index[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int i = N * threadIdx.x + e;
+        if (nucleus && i > 0 && static_cast<double>(before) >= want_p * static_cast<double>(total_k)) mine[e] = 0;
+        else before += mine[e];
+        index[e] = i < n ? ~static_cast<uint32_t>(sm.sorted[i]) : 0;
+        if (mine[e] > 0) atomicAdd(&sm.bucket[index[e] / range], mine[e]);
+      }
+      __syncthreads();
+      const u64 here = sm.bucket[threadIdx.x];
       u64 kept;
-      const u64 cum = block_scan(w, sm, kept);
-      const u64 target = static_cast<u64>(u * static_cast<double>(kept));
-      const u64 goal = target < kept ? target : kept - 1;
-      if (w > 0 && cum > goal && cum - w <= goal) a.out[r] = static_cast<long long>(sm.list[i] >> 32);
+      const u64 upto = block_scan(here, sm, kept);
+      const u64 target = static_cast<u64>(u * static_cast<double>(kept)), goal = target < kept ? target : kept - 1;
+      if (upto > goal && upto - here <= goal) sm.bin = threadIdx.x, sm.below = upto - here;
+      __syncthreads();
+      const unsigned bucket = sm.bin;
+      const u64 base = sm.below;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (mine[e] > 0 && index[e] / range == bucket) {
+          const unsigned at = atomicAdd(&sm.n, 1u);
+          sm.list[at] = index[e], sm.list_mass[at] = mine[e];
+        }
+      __syncthreads();
+      const int members = static_cast<int>(sm.n);
+      for (int i = threadIdx.x; i < members; i += kThreads) {
+        u64 cum = base;
+        for (int j = 0; j < members; ++j)
+          if (sm.list[j] < sm.list[i]) cum += sm.list_mass[j];
+        if (cum <= goal && cum + sm.list_mass[i] > goal) a.out[r] = static_cast<long long>(sm.list[i]);
+      }
       return;
     }
 
-    // ---- the long way: thresholds by narrowing histograms
-    auto passes_min_p = [&](float z) { return min_p <= 0.0f || z == zmax || ex.p(z) >= pmin; };
+    // ---- the long way: thresholds by histograms of counts and masses
     if (above_k < static_cast<u64>(k) && total > static_cast<u64>(k)) {
-      auto in_bin = [&](int, float z, uint32_t) { return z >= ex.z_cut && bin_of(z) == bin_k; };
-      const uint32_t key = key_search(sm, row, order_key(ex.z_cut), max_key, static_cast<double>(k), above_k, in_bin,
+      const uint32_t key = key_search(sm, cl, row, ex, bin_of, per, static_cast<double>(k), [](int, float, uint32_t) { return true; },
                                       [](float) { return 1ull; });
       const u64 ties = static_cast<u64>(k) - sm.below;   // that many of the equals are kept
       __syncthreads();
       cut.key = key;
-      cut.last = order_search(sm, a.vocab, ties - 1, [&](int i) { return order_key(row.at(i)) == key ? 1ull : 0ull; });
+      cut.last = order_search(sm, cl, row, [&](u64) { return ties - 1; }, [&](int, float z) { return order_key(z) == key ? 1ull : 0ull; });
       if (cut.last < 0) cut.last = 0x7fffffff;
     }
     if (nucleus) {
       const Threshold top = cut;
-      auto in = [&](int i, float z, uint32_t key) { return top.keeps(key, i) && z >= ex.z_cut && passes_min_p(z); };
-      u64 mass = 0, all;
-      row.each([&](int i, float z) {
-        if (in(i, z, order_key(z))) mass += ex.mass(z);
-      });
-      block_scan(mass, sm, all);
-      const double want = want_p * static_cast<double>(all);
-      const uint32_t key = key_search(sm, row, order_key(ex.z_cut), max_key, want, 0ull, in, [&](float z) { return ex.mass(z); });
-      const u64 above = sm.below, each = ex.mass(key_value(key));
-      __syncthreads();
-      // equals are kept while the mass before them is short of `want`
-      double need = each > 0 ? ceil((want - static_cast<double>(above)) / static_cast<double>(each)) : 1.0;
-      u64 ties = need < 1.0 ? 1 : static_cast<u64>(need);
-      while (ties > 1 && static_cast<double>(above + (ties - 1) * each) >= want) --ties;
-      while (static_cast<double>(above + ties * each) < want && ties < static_cast<u64>(a.vocab)) ++ties;
-      const int last = order_search(sm, a.vocab, ties - 1, [&](int i) {
-        const float z = row.at(i);
-        return order_key(z) == key && top.keeps(key, i) ? 1ull : 0ull;
-      });
-      cut.key = key;
-      if (key != top.key || last >= 0) cut.last = last < 0 ? 0x7fffffff : last;
+      auto mass_in = [&](int i, float z) {   // of an element that top-k and min_p keep
+        if (z < ex.z_cut || !top.keeps(order_key(z), row.first + i)) return 0ull;
+        if (z == zmax) return ex.one();
+        const double p = ex.scaled(z);
+        return p < pmin ? 0ull : Exponent::whole(p);
+      };
+      double want = 0.0;
+      u64 all = 0;
+      int j = -1;
+      if (slice <= 65536) {   // a part of 16 bits cannot overflow 32
+        cl.sync();
+        for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.limb[0][0])[i] = 0;
+        __syncthreads();
+        row.each([&](int i, float z) {
+          const u64 m = mass_in(i, z);
+          if (m == 0) return;
+          const int bin = bin_of(z);
+          atomicAdd(&sm.limb[0][bin], static_cast<unsigned>(m) & 0xffffu);
+          atomicAdd(&sm.limb[1][bin], static_cast<unsigned>(m >> 16) & 0xffffu);
+          atomicAdd(&sm.limb[2][bin], static_cast<unsigned>(m >> 32));
+        });
+        cl.sync();
+        u64 y[kPerThread];
+        cluster_counts(sm, cl, sm.limb[2], x);
+        cluster_counts(sm, cl, sm.limb[1], y);
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) x[i] = (x[i] << 16) + y[i];
+        cluster_counts(sm, cl, sm.limb[0], y);
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) x[i] = (x[i] << 16) + y[i];
+        first_reaching(sm, x, 0, [&](u64 sum) { return want = want_p * static_cast<double>(sum); }, all);
+        j = sm.bin;
+        const u64 above = sm.below;
+        __syncthreads();
+        // the bin's elements, ranked in the first CTA: the last one with less than `want` before it is the last to be kept
+        if (j >= 0) {
+          row.each([&](int i, float z) {
+            if (z < ex.z_cut || bin_of(z) != j || mass_in(i, z) == 0) return;
+            const u64 e = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
+            const unsigned at = cl.size == 1 ? atomicAdd(&sm.n, 1u) : add_peer_u32(cl.peer(&sm.n, 0), 1u);
+            if (at >= static_cast<unsigned>(kList)) return;
+            if (cl.size == 1) sm.list[at] = e;
+            else st_peer_u64(cl.peer(sm.list, 0) + at * 8, e);
+          });
+          cl.sync();
+          if (cl.rank == 0) {
+            const int n = static_cast<int>(sm.n);
+            if (threadIdx.x == 0) sm.cut_last = kNoList;
+            __syncthreads();
+            if (n <= kList) {
+              for (int i = threadIdx.x; i < n; i += kThreads) {
+                const u64 e = sm.list[i];
+                int rank = 0;
+                for (int o = 0; o < n; ++o) rank += sm.list[o] > e;
+                sm.sorted[rank] = e;
+              }
+              __syncthreads();
+              constexpr int N = kList / kThreads;
+              u64 mine[N], sum = 0, dummy;
+#pragma unroll
+              for (int e = 0; e < N; ++e) {
+                const int i = N * threadIdx.x + e;
+                mine[e] = i < n ? ex.mass(key_value(static_cast<uint32_t>(sm.sorted[i] >> 32))) : 0;
+                sum += mine[e];
+              }
+              u64 before = block_scan(sum, sm, dummy) - sum + above;
+#pragma unroll
+              for (int e = 0; e < N; ++e) {
+                const int i = N * threadIdx.x + e;
+                const bool keep = i < n && static_cast<double>(before) < want;
+                before += mine[e];
+                const bool next = i + 1 < n && static_cast<double>(before) < want;
+                if (keep && !next) {
+                  sm.cut_key = static_cast<uint32_t>(sm.sorted[i] >> 32);
+                  sm.cut_last = static_cast<int>(~static_cast<uint32_t>(sm.sorted[i]));
+                }
+              }
+            }
+            __syncthreads();
+            if (threadIdx.x > 0 && static_cast<int>(threadIdx.x) < cl.size) {
+              st_peer_u32(cl.peer(&sm.cut_key, threadIdx.x), sm.cut_key);
+              st_peer_u32(cl.peer(&sm.cut_last, threadIdx.x), static_cast<uint32_t>(sm.cut_last));
+            }
+          }
+          cl.sync();
+          if (sm.cut_last != kNoList) cut.key = sm.cut_key, cut.last = sm.cut_last;
+          else j = -2;   // more equal or nearly equal logits than the list holds
+        }
+      } else {
+        j = -2;
+      }
+      if (j == -2) {
+        auto in = [&](int i, float z, uint32_t) { return mass_in(i, z) > 0; };
+        u64 mass = 0, b, m;
+        row.each([&](int i, float z) { mass += mass_in(i, z); });
+        all = cluster_sum(mass, sm, cl, b, m);
+        want = want_p * static_cast<double>(all);
+        const uint32_t key = key_search(sm, cl, row, ex, bin_of, per, want, in, [&](float z) { return ex.mass(z); });
+        const u64 above = sm.below, each = ex.mass(key_value(key));
+        __syncthreads();
+        if (above < all) {   // (else rounding took `want` past the total: nothing is cut)
+          // equals are kept while the mass before them is short of `want`
+          const double need = each > 0 ? ceil((want - static_cast<double>(above)) / static_cast<double>(each)) : 1.0;
+          u64 ties = need < 1.0 ? 1 : static_cast<u64>(need);
+          while (ties > 1 && static_cast<double>(above + (ties - 1) * each) >= want) --ties;
+          while (static_cast<double>(above + ties * each) < want && ties < static_cast<u64>(a.vocab)) ++ties;
+          const int last = order_search(sm, cl, row, [&](u64) { return ties - 1; }, [&](int i, float z) {
+            return order_key(z) == key && top.keeps(key, row.first + i) ? 1ull : 0ull;
+          });
+          if (last >= 0) cut.last = last;
+          else if (key != top.key) cut.last = 0x7fffffff;
+          cut.key = key;
+        }
+      }
     }
   }
 
   // ---- the draw, over the vocabulary
-  auto weight = [&](int i) {
-    const float z = row.at(i);
-    if (z < ex.z_cut || !cut.keeps(order_key(z), i)) return 0ull;
-    if (z == zmax) return 1ull << ex.fraction;
-    const double p = ex.p(z);
-    return min_p > 0.0f && p < pmin ? 0ull : ex.mass_of(p);
-  };
-  u64 mass = 0, kept;
-  for (int i = threadIdx.x; i < a.vocab; i += kThreads) mass += weight(i);
-  block_scan(mass, sm, kept);
-  const u64 target = static_cast<u64>(u * static_cast<double>(kept));
-  const int token = order_search(sm, a.vocab, target < kept ? target : kept - 1, weight);
-  if (threadIdx.x == 0) a.out[r] = token;
+  const int token = order_search(sm, cl, row,
+                                 [&](u64 kept) {
+                                   const u64 target = static_cast<u64>(u * static_cast<double>(kept));
+                                   return target < kept ? target : kept - 1;
+                                 },
+                                 [&](int i, float z) {
+                                   if (z < ex.z_cut || !cut.keeps(order_key(z), row.first + i)) return 0ull;
+                                   if (z == zmax) return ex.one();
+                                   const double p = ex.scaled(z);
+                                   return p < pmin ? 0ull : Exponent::whole(p);
+                                 });
+  if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = token;
+}
+
+template <class T>
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t s) {
+  // Enough CTAs for two per SM where rows are few, and slices that leave room for two CTAs' on an SM; a vocabulary that
+  // does not fit eight SMs' shared memory is read from global memory in every pass.
+  constexpr int kFixed = (sizeof(Shared) + 15) / 16 * 16 + 16, kHalf = 113 * 1024, kWhole = 227 * 1024;
+  int c = 1;
+  while (c < kMaxCluster && (static_cast<long long>(a.rows) * c < 148 || static_cast<long long>(a.vocab) * sizeof(T) / c > kHalf - kFixed - 64)) c *= 2;
+  constexpr int E = 16 / sizeof(T);
+  const int slice = static_cast<int>(((static_cast<long long>(a.vocab) + c - 1) / c + E - 1) / E * E);
+  const bool staged = static_cast<long long>(slice) * sizeof(T) + kFixed <= kWhole;
+  const size_t smem = kFixed + (staged ? static_cast<size_t>(slice) * sizeof(T) : 0);
+  static std::atomic<unsigned long long> configured{0};   // one bit per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if ((configured.load(std::memory_order_relaxed) & bit) == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWhole);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * c);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, a, c, slice, static_cast<int>(staged));
 }
 
 }  // namespace
 
 const char* sample_rows(const SampleArgs& a, cudaStream_t s) {
   if (a.rows == 0) return nullptr;
-  if (a.bf16) sample_rows_kernel<__nv_bfloat16><<<a.rows, kThreads, 0, s>>>(a);
-  else sample_rows_kernel<float><<<a.rows, kThreads, 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  if (static_cast<long long>(a.rows) * kMaxCluster >= (1LL << 31)) return "sample_rows: too many rows";
+  const cudaError_t e = a.bf16 ? launch_sample<__nv_bfloat16>(a, s) : launch_sample<float>(a, s);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
