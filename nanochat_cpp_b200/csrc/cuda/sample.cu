@@ -49,14 +49,16 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// This CTA's slice of the row: elements [0, n) stand for indices `first` + i. `p` is in shared or global memory.
-template <class T>
+// This CTA's slice of the row: elements [0, n) stand for indices `first` + i. In global memory (RAW) they are as the
+// caller left them, in shared memory they have been cleaned.
+template <class T, bool RAW>
 struct Slice {
   const T* p;
   int n, first;
+  __device__ __forceinline__ static float as_is(float z) { return RAW ? clean(z) : z; }
   __device__ __forceinline__ float at(int i) const {
-    if constexpr (sizeof(T) == 2) return clean(__bfloat162float(p[i]));
-    else return clean(p[i]);
+    if constexpr (sizeof(T) == 2) return as_is(__bfloat162float(p[i]));
+    else return as_is(p[i]);
   }
   template <class F>
   __device__ __forceinline__ static void spread(const uint4& w, int i, F f) {
@@ -66,7 +68,7 @@ struct Slice {
       float z;
       if constexpr (sizeof(T) == 2) z = __uint_as_float((e & 1) ? (u[e / 2] & 0xffff0000u) : (u[e / 2] << 16));
       else z = __uint_as_float(u[e]);
-      f(i + e, clean(z));
+      f(i + e, as_is(z));
     }
   }
   // f(i, z) for every element, by 16-byte loads between the first and the last aligned address
@@ -83,6 +85,17 @@ struct Slice {
   }
 };
 
+// 2^(j / 32)
+__device__ const double kPowers[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
 // Mass of a logit: exp((z - zmax) / t) in 64 bits, as an integer in units of 2^-fraction. With y = (z - zmax) / t * 32 / ln 2
 // split into a whole number k and r in [-1/2, 1/2], p = 2^(k / 32) * 2^(r / 32): the first from a table of 32 and the
 // exponent field, the second by its Taylor polynomial to the fourth power (remainder below 2^-39 of p).
@@ -91,10 +104,10 @@ struct Exponent {
   const double* table;   // shared: 2^(j / 32)
   float z_max, z_cut;    // z_cut: below there is no mass
   int fraction;
-  __device__ __forceinline__ double scaled(float z) const {   // p * 2^fraction, z_cut <= z
+  __device__ __forceinline__ double scaled(float z) const {   // p * 2^fraction, z_cut <= z; exactly 2^fraction at the maximum
     constexpr double kShift = 6755399441055744.0;              // 1.5 * 2^52: adding it leaves the whole number in the low bits
     constexpr double kLn = 0.021660849392498290;               // ln 2 / 32
-    const double d = static_cast<double>(z) - zmax;
+    const double d = static_cast<double>(fminf(z, 3.402823466e38f)) - zmax;
     const double kd = fma(d, per, kShift);
     const int k = __double2loint(kd);
     const double r = fma(d, per, -(kd - kShift));
@@ -106,7 +119,7 @@ struct Exponent {
     return static_cast<u64>(__double_as_longlong(m + 4503599627370496.0)) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ u64 one() const { return 1ull << fraction; }
-  __device__ __forceinline__ u64 mass(float z) const { return z < z_cut ? 0ull : z == z_max ? one() : whole(scaled(z)); }
+  __device__ __forceinline__ u64 mass(float z) const { return z < z_cut ? 0ull : whole(scaled(z)); }
 };
 
 struct Shared {
@@ -125,9 +138,8 @@ struct Shared {
   u64 sums[2];                 // this CTA's totals, read by the others (two, used in turn)
   float warp_max[kWarps], warp_min[kWarps];
   int warp_arg[kWarps];
-  float top, bottom;           // of this CTA's slice
-  int arg;
-  unsigned n;                  // candidates collected
+  u64 best[2];                 // of this CTA's slice: largest and smallest logit, index of the largest
+  alignas(8) unsigned n;       // candidates collected
   int bin;
   u64 below, inside;
   int lo, hi;
@@ -153,21 +165,8 @@ __device__ __forceinline__ u64 ld_peer_u64(uint32_t at) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t ld_peer_u32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_peer_u64(uint32_t at, u64 v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
-}
 __device__ __forceinline__ void st_peer_u32(uint32_t at, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t add_peer_u32(uint32_t at, uint32_t v) {
-  uint32_t old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(at), "r"(v) : "memory");
-  return old;
 }
 
 __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {   // inclusive
@@ -196,6 +195,18 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& sm, u64& total) {
   return v + (warp > 0 ? before : 0);
 }
 
+// Sum over the CTAs of the cluster of a 64-bit word of their shared memory: every read is issued before any is used
+// (ranks past the cluster read this CTA's own, and count for nothing).
+template <int N>
+__device__ __forceinline__ void read_peers(const Cluster& cl, const u64* at, u64 (&v)[kMaxCluster][N]) {
+#pragma unroll
+  for (int r = 0; r < kMaxCluster; ++r) {
+    const uint32_t p = cl.peer(at, r < cl.size ? r : cl.rank);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[r][i] = ld_peer_u64(p + 8 * i);
+  }
+}
+
 // The sum of one value per thread over the cluster; `before` is the part of CTAs of lower rank, `mine` this CTA's.
 __device__ __forceinline__ u64 cluster_sum(u64 v, Shared& sm, Cluster& cl, u64& before, u64& mine) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -209,53 +220,59 @@ __device__ __forceinline__ u64 cluster_sum(u64 v, Shared& sm, Cluster& cl, u64& 
   cl.turn ^= 1;   // the slot of the turn before may still be read
   if (threadIdx.x == 0) sm.sums[cl.turn] = mine;
   cl.sync();
-  u64 all = 0;
+  u64 all = 0, peers[kMaxCluster][1];
+  read_peers(cl, &sm.sums[cl.turn], peers);
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r)
-    if (r < cl.size) {
-      const u64 x = ld_peer_u64(cl.peer(&sm.sums[cl.turn], r));
-      if (r < cl.rank) before += x;
-      all += x;
-    }
+  for (int r = 0; r < kMaxCluster; ++r) {
+    before += r < cl.rank ? peers[r][0] : 0;
+    all += r < cl.size ? peers[r][0] : 0;
+  }
   return all;
-}
-
-// f(rank) for every CTA of the cluster, unrolled so that the reads of all of them are in flight together
-template <class F>
-__device__ __forceinline__ void each_peer(const Cluster& cl, F f) {
-#pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r)
-    if (r < cl.size) f(r);
 }
 
 // The bins of all CTAs, kPerThread neighbouring ones per thread.
 __device__ __forceinline__ void cluster_bins(Shared& sm, const Cluster& cl, u64 (&x)[kPerThread]) {
   cl.sync();
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = 0;
-  each_peer(cl, [&](int r) {
-    const uint32_t at = cl.peer(&sm.hist[kPerThread * threadIdx.x], r);
+  for (int i = 0; i < kPerThread; ++i) x[i] = sm.hist[kPerThread * threadIdx.x + i];
+  if (cl.size == 1) return;
+  u64 v[kMaxCluster][kPerThread];
+  read_peers(cl, &sm.hist[kPerThread * threadIdx.x], v);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) x[i] += ld_peer_u64(at + 8 * i);
-  });
+  for (int i = 0; i < kPerThread; ++i) {
+    x[i] = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) x[i] += r < cl.size ? v[r][i] : 0;
+  }
 }
 __device__ __forceinline__ void cluster_counts(Shared& sm, const Cluster& cl, const unsigned* bins, u64 (&x)[kPerThread]) {
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = 0;
-  each_peer(cl, [&](int r) {
-    const uint32_t at = cl.peer(&bins[kPerThread * threadIdx.x], r);
+  for (int i = 0; i < kPerThread; ++i) x[i] = bins[kPerThread * threadIdx.x + i];
+  if (cl.size == 1) return;
+  u64 v[kMaxCluster][kPerThread / 2];
+  read_peers(cl, reinterpret_cast<const u64*>(&bins[kPerThread * threadIdx.x]), v);
 #pragma unroll
-    for (int i = 0; i < kPerThread; i += 2) {
-      const u64 two = ld_peer_u64(at + 4 * i);
-      x[i] += two & 0xffffffffu, x[i + 1] += two >> 32;
-    }
-  });
+  for (int i = 0; i < kPerThread; ++i) {
+    x[i] = 0;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) x[i] += r < cl.size ? (v[r][i / 2] >> (32 * (i & 1))) & 0xffffffffu : 0;
+  }
+}
+
+// Candidates that every CTA has collected in its own list, read by the first CTA: f(candidate), each once.
+template <class F>
+__device__ __forceinline__ void pull_lists(Shared& sm, const Cluster& cl, F f) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = warp % cl.size;   // the warps share out the lists
+  const int n = min(static_cast<int>(ld_peer_u64(cl.peer(&sm.n, r)) & 0xffffffffu), kList);
+  const uint32_t list = cl.peer(sm.list, r);
+#pragma unroll 2
+  for (int i = warp / cl.size * 32 + lane; i < n; i += kWarps / cl.size * 32) f(ld_peer_u64(list + 8 * i));
 }
 
 // The first index at which the running weight (vocabulary order) exceeds target_of(total weight), or -1; w(i, z) is the
 // weight of element i of the slice. The CTA that holds it divides its slice among its warps until one warp can walk it.
-template <class T, class Target, class W>
-__device__ int order_search(Shared& sm, Cluster& cl, const Slice<T>& row, Target target_of, W w) {
+template <class S, class Target, class W>
+__device__ int order_search(Shared& sm, Cluster& cl, const S& row, Target target_of, W w) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 s = 0, before, mine;
   // the first division is by slices of the CTAs and, inside, by sixteenths for its warps
@@ -263,8 +280,17 @@ __device__ int order_search(Shared& sm, Cluster& cl, const Slice<T>& row, Target
   int seg = ((row.n + kWarps - 1) / kWarps + 31) / 32 * 32;
   {
     const int a = min(warp * seg, hi), b = min(a + seg, hi);
-#pragma unroll 4
-    for (int i = a + lane; i < b; i += 32) s += w(i, row.at(i));
+    int i = a + lane;
+    for (; i + 96 < b; i += 128) {
+      float z[4];
+      u64 m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = row.at(i + 32 * e);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m[e] = w(i + 32 * e, z[e]);
+      s += (m[0] + m[1]) + (m[2] + m[3]);
+    }
+    for (; i < b; i += 32) s += w(i, row.at(i));
   }
   u64 target = target_of(cluster_sum(s, sm, cl, before, mine));
   const bool here = target >= before && target - before < mine;
@@ -335,11 +361,11 @@ __device__ __forceinline__ u64 first_reaching(Shared& sm, const u64 (&x)[kPerThr
   for (int i = 0; i < kPerThread; ++i) sum += x[i];
   if (threadIdx.x == 0) sm.bin = -1;
   const u64 start = block_scan(sum, sm, total) + above - sum;
-  const double want = want_of(total);
+  const u64 want = static_cast<u64>(ceil(want_of(total)));   // a whole weight reaches it exactly if it reaches the real number
   u64 c = start;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    if (static_cast<double>(c) < want && static_cast<double>(c + x[i]) >= want) sm.bin = kPerThread * threadIdx.x + i, sm.below = c;
+    if (c < want && c + x[i] >= want) sm.bin = kPerThread * threadIdx.x + i, sm.below = c;
     c += x[i];
   }
   __syncthreads();
@@ -349,8 +375,8 @@ __device__ __forceinline__ u64 first_reaching(Shared& sm, const u64 (&x)[kPerThr
 // Descending search among the elements that `in` selects: the largest key at which the running weight (from the top) reaches
 // `want` > 0. First over the bins of z, then over the bits of the keys inside the bin. On return sm.below is the
 // weight strictly above that key.
-template <class T, class Bin, class In, class W>
-__device__ uint32_t key_search(Shared& sm, Cluster& cl, const Slice<T>& row, const Exponent& ex, Bin bin_of, float per, double want, In in, W w) {
+template <class S, class Bin, class In, class W>
+__device__ uint32_t key_search(Shared& sm, Cluster& cl, const S& row, const Exponent& ex, Bin bin_of, float per, double want, In in, W w) {
   uint32_t lo = order_key(ex.z_cut), hi = order_key(ex.z_max);
   u64 above = 0, total, x[kPerThread];
   int bin = -1;
@@ -383,7 +409,7 @@ __device__ uint32_t key_search(Shared& sm, Cluster& cl, const Slice<T>& row, con
     if (first) {
       // the keys that the bin can hold: a hundredth of a bin more on either side, far above the rounding of bin_of
       bin = j;
-      const float z_lo = ex.z_max - (j + 1.01f) / per, z_hi = ex.z_max - (j - 0.01f) / per;
+      const float z_lo = ex.z_max - (j + 0.51f) / per, z_hi = ex.z_max - (j - 0.51f) / per;
       if (per < 1e30f && z_lo > ex.z_cut && j < kBins - 1) lo = order_key(z_lo);
       if (per < 1e30f && z_hi < ex.z_max) hi = order_key(z_hi);
     } else {
@@ -398,27 +424,30 @@ __device__ uint32_t key_search(Shared& sm, Cluster& cl, const Slice<T>& row, con
   return lo;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleArgs a, int cluster, int slice, int staged) {
+template <class T, bool STAGED>
+__global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleArgs a, int cluster, int slice) {
   extern __shared__ __align__(16) uint8_t dyn[];
   Shared& sm = *reinterpret_cast<Shared*>(dyn);
   Cluster cl;
   cl.size = cluster, cl.rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0, cl.turn = 0;
   const int r = blockIdx.x / cluster, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Slice<T> row;
+  Slice<T, !STAGED> row;
   row.first = min(cl.rank * slice, a.vocab);
   row.n = min(slice, a.vocab - row.first);
-  const Slice<T> global{static_cast<const T*>(a.logits) + r * a.ld + row.first, row.n, row.first};
+  const Slice<T, true> global{static_cast<const T*>(a.logits) + r * a.ld + row.first, row.n, row.first};
   const float t = a.temperature_rows != nullptr ? a.temperature_rows[r] : a.temperature;
   const float top_p = a.top_p_rows != nullptr ? a.top_p_rows[r] : a.top_p;
   const float min_p = a.min_p_rows != nullptr ? a.min_p_rows[r] : a.min_p;
   int k = a.top_k_rows != nullptr ? a.top_k_rows[r] : a.top_k;
   if (k <= 0 || k > a.vocab) k = a.vocab;
+  if (threadIdx.x < 32) sm.table[threadIdx.x] = kPowers[threadIdx.x];
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sm.count[i] = 0;
+  if (threadIdx.x == 0) sm.n = 0;
 
   // ---- the largest logit (lowest index of equals) and the smallest above -infinity; the slice goes to shared memory
   // with the alignment that it has, so that 16-byte pieces stay 16-byte pieces
   T* stage = reinterpret_cast<T*>(dyn + (sizeof(Shared) + 15) / 16 * 16) + (reinterpret_cast<uintptr_t>(global.p) & 15) / sizeof(T);
-  row.p = staged ? stage : global.p;
+  row.p = STAGED ? stage : global.p;
   float zmax = -CUDART_INF_F, zmin = CUDART_INF_F;
   int arg = 0x7fffffff;
   {
@@ -429,20 +458,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
       if (z > zmax || (z == zmax && i < arg)) zmax = z, arg = i;
       if (z > -CUDART_INF_F) zmin = fminf(zmin, z);
     };
-    if (threadIdx.x < head) {
-      if (staged) stage[threadIdx.x] = global.p[threadIdx.x];
-      see(threadIdx.x, global.at(threadIdx.x));
-    }
+    auto keep = [&](int i, float z) {
+      see(i, z);
+      if constexpr (STAGED) stage[i] = static_cast<T>(z);   // (exact: a bf16 value, or fp32)
+    };
+    if (threadIdx.x < head) keep(threadIdx.x, global.at(threadIdx.x));
 #pragma unroll 4
     for (int v = threadIdx.x; v < vecs; v += kThreads) {
-      const uint4 x = __ldcs(reinterpret_cast<const uint4*>(global.p + head + v * E));
-      if (staged) *reinterpret_cast<uint4*>(stage + head + v * E) = x;
-      Slice<T>::spread(x, head + v * E, see);
+      const int i0 = head + v * E;
+      uint4 x = __ldcs(reinterpret_cast<const uint4*>(global.p + i0));
+      float z[E];
+      Slice<T, true>::spread(x, 0, [&](int e, float c) { z[e] = c; });
+#pragma unroll
+      for (int e = 0; e < E; ++e) see(i0 + e, z[e]);
+      if constexpr (STAGED) {
+        if constexpr (E == 4)
+          x = make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
+        else
+          x = make_uint4(pack_bf16(z[0], z[1]), pack_bf16(z[2], z[3]), pack_bf16(z[E - 4], z[E - 3]), pack_bf16(z[E - 2], z[E - 1]));
+        *reinterpret_cast<uint4*>(stage + i0) = x;
+      }
     }
-    for (int i = head + vecs * E + threadIdx.x; i < row.n; i += kThreads) {
-      if (staged) stage[i] = global.p[i];
-      see(i, global.at(i));
-    }
+    for (int i = head + vecs * E + threadIdx.x; i < row.n; i += kThreads) keep(i, global.at(i));
   }
   if (arg != 0x7fffffff) arg += row.first;
   auto take = [&](float oz, int oi, float om) {
@@ -453,21 +490,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
   for (int o = 16; o > 0; o >>= 1)
     take(__shfl_xor_sync(0xffffffffu, zmax, o), __shfl_xor_sync(0xffffffffu, arg, o), __shfl_xor_sync(0xffffffffu, zmin, o));
   if (lane == 0) sm.warp_max[warp] = zmax, sm.warp_arg[warp] = arg, sm.warp_min[warp] = zmin;
-  if (threadIdx.x < 32) sm.table[threadIdx.x] = exp2(threadIdx.x / 32.0);
-  for (int i = threadIdx.x; i < kBins; i += kThreads) sm.count[i] = 0;
-  if (threadIdx.x == 0) sm.n = 0;
   __syncthreads();
   zmax = sm.warp_max[lane % kWarps], arg = sm.warp_arg[lane % kWarps], zmin = sm.warp_min[lane % kWarps];
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1)
     take(__shfl_xor_sync(0xffffffffu, zmax, o), __shfl_xor_sync(0xffffffffu, arg, o), __shfl_xor_sync(0xffffffffu, zmin, o));
   if (cl.size > 1) {
-    if (threadIdx.x == 0) sm.top = zmax, sm.arg = arg, sm.bottom = zmin;
+    if (threadIdx.x == 0) {
+      sm.best[0] = static_cast<u64>(__float_as_uint(zmax)) << 32 | __float_as_uint(zmin);
+      sm.best[1] = static_cast<unsigned>(arg);
+    }
     cl.sync();
-    each_peer(cl, [&](int c) {
-      take(__uint_as_float(ld_peer_u32(cl.peer(&sm.top, c))), static_cast<int>(ld_peer_u32(cl.peer(&sm.arg, c))),
-           __uint_as_float(ld_peer_u32(cl.peer(&sm.bottom, c))));
-    });
+    u64 v[kMaxCluster][2];
+    read_peers(cl, sm.best, v);   // (this CTA's own again where the cluster is smaller)
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      take(__uint_as_float(static_cast<uint32_t>(v[c][0] >> 32)), static_cast<int>(v[c][1]), __uint_as_float(static_cast<uint32_t>(v[c][0])));
   }
   if (zmax == -CUDART_INF_F || !(t > 0.0f) || k == 1 || !(top_p > 0.0f) || !(min_p <= 1.0f)) {
     if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = zmax == -CUDART_INF_F ? -1 : arg;
@@ -475,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
     return;
   }
   Exponent ex;
-  ex.zmax = static_cast<double>(zmax), ex.z_max = zmax, ex.table = sm.table;
+  ex.zmax = static_cast<double>(fminf(zmax, 3.402823466e38f)), ex.z_max = zmax, ex.table = sm.table;
   ex.per = 46.166241308446828384 / static_cast<double>(t);
   int log_v = 0;
   while ((1ll << log_v) < a.vocab) ++log_v;
@@ -489,8 +527,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
   cut.key = order_key(ex.z_cut);
   if (filtered) {
     const float width = fminf(zmax - zmin, kReach * t);
-    const float per = width > 0.0f ? static_cast<float>(kBins) / width : 0.0f;
-    auto bin_of = [&](float z) { return z == zmax ? 0 : min(static_cast<int>((zmax - z) * per), kBins - 1); };
+    const float per = width > 0.0f ? fminf(static_cast<float>(kBins) / width, 1e37f) : 0.0f;
+    // the nearest whole number to (zmax - z) * per, left in the low bits by adding 2^23
+    auto bin_of = [&](float z) { return min(__float_as_int(fmaf(zmax - z, per, 8388608.0f)) & 0x7fffff, kBins - 1); };
     row.each([&](int, float z) {
       if (z >= ex.z_cut) atomicAdd(&sm.count[bin_of(z)], 1u);
     });
@@ -519,26 +558,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
 
     if (n_cut <= kList) {
       // ---- the short way, in the first CTA: candidates go to their bin's places, are ranked inside it, and decided on
+      const float z_lo = bin_cut < kBins - 1 && per < 1e30f ? fmaxf(zmax - (bin_cut + 0.51f) / per, ex.z_cut) : ex.z_cut;
       row.each([&](int i, float z) {
-        if (z < ex.z_cut) return;
+        if (z < z_lo) return;
         const int bin = bin_of(z);
         if (bin > bin_cut) return;
-        const u64 e = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
-        if (cl.size == 1) sm.list[atomicAdd(&sm.cursor[bin], 1u)] = e;
-        else st_peer_u64(cl.peer(sm.list, 0) + add_peer_u32(cl.peer(&sm.cursor[bin], 0), 1u) * 8, e);
+        sm.list[atomicAdd(&sm.n, 1u)] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
       });
+      cl.sync();
+      if (cl.rank == 0)
+        pull_lists(sm, cl, [&](u64 e) {
+          sm.sorted[atomicAdd(&sm.cursor[bin_of(key_value(static_cast<uint32_t>(e >> 32)))], 1u)] = e;
+        });
       cl.sync();
       if (cl.rank != 0) return;   // nobody reads this CTA's memory any more
       const int n = static_cast<int>(n_cut);
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        const u64 e = sm.list[i];
+        const u64 e = sm.sorted[i];
         const int bin = bin_of(key_value(static_cast<uint32_t>(e >> 32)));
         const int from = bin > 0 ? sm.cursor[bin - 1] : 0, to = sm.cursor[bin];
         int rank = from;
-        for (int j = from; j < to; ++j) rank += sm.list[j] > e;
-        sm.sorted[rank] = e;
+        for (int j = from; j < to; ++j) rank += sm.sorted[j] > e;
+        sm.list[rank] = e;
       }
       sm.bucket[threadIdx.x] = 0;
+      if (threadIdx.x == 0) sm.n = 0;
       __syncthreads();
       // two neighbours per thread
       constexpr int N = kList / kThreads;
@@ -548,8 +592,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         const int i = N * threadIdx.x + e;
         mine[e] = 0;
         if (i < n && i < k) {
-          const float z = key_value(static_cast<uint32_t>(sm.sorted[i] >> 32));
-          const double p = z == zmax ? static_cast<double>(ex.one()) : ex.scaled(z);
+          const float z = key_value(static_cast<uint32_t>(sm.list[i] >> 32));
+          const double p = ex.scaled(z);
           if (i == 0 || p >= pmin) mine[e] = Exponent::whole(p);
         }
         sum += mine[e];
@@ -564,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         const int i = N * threadIdx.x + e;
         if (nucleus && i > 0 && static_cast<double>(before) >= want_p * static_cast<double>(total_k)) mine[e] = 0;
         else before += mine[e];
-        index[e] = i < n ? ~static_cast<uint32_t>(sm.sorted[i]) : 0;
+        index[e] = i < n ? ~static_cast<uint32_t>(sm.list[i]) : 0;
         if (mine[e] > 0) atomicAdd(&sm.bucket[index[e] / range], mine[e]);
       }
       __syncthreads();
@@ -580,15 +624,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
       for (int e = 0; e < N; ++e)
         if (mine[e] > 0 && index[e] / range == bucket) {
           const unsigned at = atomicAdd(&sm.n, 1u);
-          sm.list[at] = index[e], sm.list_mass[at] = mine[e];
+          sm.sorted[at] = index[e], sm.list_mass[at] = mine[e];
         }
       __syncthreads();
       const int members = static_cast<int>(sm.n);
       for (int i = threadIdx.x; i < members; i += kThreads) {
         u64 cum = base;
         for (int j = 0; j < members; ++j)
-          if (sm.list[j] < sm.list[i]) cum += sm.list_mass[j];
-        if (cum <= goal && cum + sm.list_mass[i] > goal) a.out[r] = static_cast<long long>(sm.list[i]);
+          if (sm.sorted[j] < sm.sorted[i]) cum += sm.list_mass[j];
+        if (cum <= goal && cum + sm.list_mass[i] > goal) a.out[r] = static_cast<long long>(sm.sorted[i]);
       }
       return;
     }
@@ -605,11 +649,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
     }
     if (nucleus) {
       const Threshold top = cut;
-      auto mass_in = [&](int i, float z) {   // of an element that top-k and min_p keep
-        if (z < ex.z_cut || !top.keeps(order_key(z), row.first + i)) return 0ull;
-        if (z == zmax) return ex.one();
-        const double p = ex.scaled(z);
-        return p < pmin ? 0ull : Exponent::whole(p);
+      auto mass_in = [&](int i, float z) {   // of an element that top-k and min_p keep; no branches, so that several overlap
+        const bool keep = z >= ex.z_cut && top.keeps(order_key(z), row.first + i);
+        const double p = ex.scaled(fmaxf(z, ex.z_cut));
+        const u64 m = Exponent::whole(p);
+        return keep && p >= pmin ? m : 0ull;
       };
       double want = 0.0;
       u64 all = 0;
@@ -619,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.limb[0][0])[i] = 0;
         __syncthreads();
         row.each([&](int i, float z) {
+          if (z < ex.z_cut) return;
           const u64 m = mass_in(i, z);
           if (m == 0) return;
           const int bin = bin_of(z);
@@ -641,25 +686,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         __syncthreads();
         // the bin's elements, ranked in the first CTA: the last one with less than `want` before it is the last to be kept
         if (j >= 0) {
+          const bool narrow = per < 1e30f;   // (bounds a hundredth of a bin wide of it)
+          const float z_lo = narrow && j < kBins - 1 ? fmaxf(zmax - (j + 0.51f) / per, ex.z_cut) : ex.z_cut;
+          const float z_hi = narrow && j > 0 ? zmax - (j - 0.51f) / per : zmax;
           row.each([&](int i, float z) {
-            if (z < ex.z_cut || bin_of(z) != j || mass_in(i, z) == 0) return;
-            const u64 e = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
-            const unsigned at = cl.size == 1 ? atomicAdd(&sm.n, 1u) : add_peer_u32(cl.peer(&sm.n, 0), 1u);
-            if (at >= static_cast<unsigned>(kList)) return;
-            if (cl.size == 1) sm.list[at] = e;
-            else st_peer_u64(cl.peer(sm.list, 0) + at * 8, e);
+            if (z < z_lo || z > z_hi || bin_of(z) != j || mass_in(i, z) == 0) return;
+            const unsigned at = atomicAdd(&sm.n, 1u);
+            if (at < static_cast<unsigned>(kList))
+              sm.list[at] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
           });
           cl.sync();
           if (cl.rank == 0) {
-            const int n = static_cast<int>(sm.n);
-            if (threadIdx.x == 0) sm.cut_last = kNoList;
+            u64 n_all = 0;
+            for (int c = 0; c < cl.size; ++c) n_all += ld_peer_u64(cl.peer(&sm.n, c)) & 0xffffffffu;
+            const int n = static_cast<int>(n_all);
+            if (threadIdx.x == 0) sm.cut_last = kNoList, sm.lo = 0;
             __syncthreads();
-            if (n <= kList) {
+            if (n_all <= kList) {
+              pull_lists(sm, cl, [&](u64 e) { sm.sorted[atomicAdd(&sm.lo, 1)] = e; });
+              __syncthreads();
               for (int i = threadIdx.x; i < n; i += kThreads) {
-                const u64 e = sm.list[i];
+                const u64 e = sm.sorted[i];
                 int rank = 0;
-                for (int o = 0; o < n; ++o) rank += sm.list[o] > e;
-                sm.sorted[rank] = e;
+                for (int o = 0; o < n; ++o) rank += sm.sorted[o] > e;
+                sm.list[rank] = e;
               }
               __syncthreads();
               constexpr int N = kList / kThreads;
@@ -667,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
 #pragma unroll
               for (int e = 0; e < N; ++e) {
                 const int i = N * threadIdx.x + e;
-                mine[e] = i < n ? ex.mass(key_value(static_cast<uint32_t>(sm.sorted[i] >> 32))) : 0;
+                mine[e] = i < n ? ex.mass(key_value(static_cast<uint32_t>(sm.list[i] >> 32))) : 0;
                 sum += mine[e];
               }
               u64 before = block_scan(sum, sm, dummy) - sum + above;
@@ -678,8 +728,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
                 before += mine[e];
                 const bool next = i + 1 < n && static_cast<double>(before) < want;
                 if (keep && !next) {
-                  sm.cut_key = static_cast<uint32_t>(sm.sorted[i] >> 32);
-                  sm.cut_last = static_cast<int>(~static_cast<uint32_t>(sm.sorted[i]));
+                  sm.cut_key = static_cast<uint32_t>(sm.list[i] >> 32);
+                  sm.cut_last = static_cast<int>(~static_cast<uint32_t>(sm.list[i]));
                 }
               }
             }
@@ -729,10 +779,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
                                    return target < kept ? target : kept - 1;
                                  },
                                  [&](int i, float z) {
-                                   if (z < ex.z_cut || !cut.keeps(order_key(z), row.first + i)) return 0ull;
-                                   if (z == zmax) return ex.one();
-                                   const double p = ex.scaled(z);
-                                   return p < pmin ? 0ull : Exponent::whole(p);
+                                   const bool keep = z >= ex.z_cut && cut.keeps(order_key(z), row.first + i);
+                                   const double p = ex.scaled(fmaxf(z, ex.z_cut));
+                                   const u64 m = Exponent::whole(p);
+                                   return keep && p >= pmin ? m : 0ull;
                                  });
   if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = token;
 }
@@ -753,7 +803,9 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t s) {
   cudaGetDevice(&dev);
   const unsigned long long bit = 1ull << (dev & 63);
   if ((configured.load(std::memory_order_relaxed) & bit) == 0) {
-    const cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWhole);
+    cudaError_t e = cudaFuncSetAttribute(sample_rows_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWhole);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(sample_rows_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWhole);
     if (e != cudaSuccess) return e;
     configured.fetch_or(bit);
   }
@@ -767,7 +819,7 @@ cudaError_t launch_sample(const SampleArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim.x = c, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, a, c, slice, static_cast<int>(staged));
+  return cudaLaunchKernelEx(&cfg, staged ? sample_rows_kernel<T, true> : sample_rows_kernel<T, false>, a, c, slice);
 }
 
 }  // namespace
