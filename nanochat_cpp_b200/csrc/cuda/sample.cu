@@ -11,7 +11,7 @@
 // A row belongs to a cluster of 1, 2, 4 or 8 CTAs (more where there are few rows); each copies its slice into shared
 // memory, so the logits are read from memory once. A histogram over z (bins of equal width below the maximum: monotone in z, and
 // spread, where the bits of z would put most logits into a handful of bins) finds a cut below which nothing can be kept. If at
-// most 1024 logits lie above it - the usual settings - they are collected in the first CTA, sorted, and
+// most 2048 logits lie above it - the usual settings - they are collected in the first CTA, sorted, and
 // everything else happens there: only these need the exponential. Otherwise the thresholds are narrowed down by
 // further histograms over the bits of z, and the draw walks the vocabulary by halving it among the warps. Bound by the
 // chain of such steps (each a pass over the slice and a cluster barrier) for few rows, by 64-bit arithmetic for many.
@@ -35,7 +35,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kPerThread = kBins / kThreads;
-constexpr int kList = 1024;      // candidates that are sorted in shared memory
+constexpr int kList = 2048;      // candidates that are sorted in shared memory
 constexpr int kMaxCluster = 8;
 constexpr float kReach = 33.0f;  // e^-33 < 2^-47: no mass beyond
 
@@ -71,17 +71,20 @@ struct Slice {
       f(i + e, as_is(z));
     }
   }
-  // f(i, z) for every element, by 16-byte loads between the first and the last aligned address
+  // f(i, z) for every element that is not below `floor`, by 16-byte loads between the first and the last aligned address
   template <class F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each(float floor, F f) const {
     constexpr int E = 16 / sizeof(T);
     const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
     const int vecs = (n - head) / E;
-    if (threadIdx.x < head) f(static_cast<int>(threadIdx.x), at(threadIdx.x));
+    auto one = [&](int i, float z) {
+      if (z >= floor) f(i, z);
+    };
+    if (threadIdx.x < head) one(static_cast<int>(threadIdx.x), at(threadIdx.x));
 #pragma unroll 2
     for (int v = threadIdx.x; v < vecs; v += kThreads)
-      spread(*reinterpret_cast<const uint4*>(p + head + v * E), head + v * E, f);
-    for (int i = head + vecs * E + threadIdx.x; i < n; i += kThreads) f(i, at(i));
+      spread(*reinterpret_cast<const uint4*>(p + head + v * E), head + v * E, one);
+    for (int i = head + vecs * E + threadIdx.x; i < n; i += kThreads) one(i, at(i));
   }
 };
 
@@ -122,23 +125,22 @@ struct Exponent {
   __device__ __forceinline__ u64 mass(float z) const { return z < z_cut ? 0ull : whole(scaled(z)); }
 };
 
-struct Shared {
+struct alignas(16) Shared {
   double table[32];
   union {
     u64 hist[kBins];           // masses or counts of this CTA, summed over the cluster by whoever reads them
     unsigned limb[3][kBins];   // masses in three parts of 16 bits (32-bit additions are native, 64-bit ones a loop)
     struct {                   // the short way, in the first CTA
-      u64 sorted[kList], list_mass[kList], bucket[kThreads];
+      u64 sorted[kList], bucket[kThreads];
     };
   };
   u64 list[kList];             // candidates: order key in the high half, ~index in the low
-  unsigned count[kBins];
-  unsigned cursor[kBins];      // the first CTA: where the next candidate of a bin goes; in the end where its last one ends
+  unsigned count[kBins];       // logits per bin; later, in the first CTA, where the bin's next candidate goes
   u64 warp_sum[kWarps];
   u64 sums[2];                 // this CTA's totals, read by the others (two, used in turn)
   float warp_max[kWarps], warp_min[kWarps];
   int warp_arg[kWarps];
-  u64 best[2];                 // of this CTA's slice: largest and smallest logit, index of the largest
+  alignas(16) u64 best[2];                 // of this CTA's slice: largest and smallest logit, index of the largest
   alignas(8) unsigned n;       // candidates collected
   int bin;
   u64 below, inside;
@@ -149,6 +151,7 @@ struct Shared {
   int cut_last;                // kNoList: too many candidates for the list
 };
 constexpr int kNoList = -2;
+static_assert(sizeof(Shared) <= 49 * 1024, "two CTAs with 64 KB of logits each share an SM");
 
 // What a CTA knows of its cluster, and the steps that need all of it.
 struct Cluster {
@@ -195,15 +198,25 @@ __device__ __forceinline__ u64 block_scan(u64 v, Shared& sm, u64& total) {
   return v + (warp > 0 ? before : 0);
 }
 
-// Sum over the CTAs of the cluster of a 64-bit word of their shared memory: every read is issued before any is used
-// (ranks past the cluster read this CTA's own, and count for nothing).
-template <int N>
-__device__ __forceinline__ void read_peers(const Cluster& cl, const u64* at, u64 (&v)[kMaxCluster][N]) {
+// N 64-bit words at `at` in every CTA of the cluster: f(rank, words). Four CTAs' reads are in flight at a time; ranks past
+// the cluster read this CTA's own words and are left out by the caller.
+template <int N, class F>
+__device__ __forceinline__ void read_peers(const Cluster& cl, const u64* at, F f) {
 #pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r) {
-    const uint32_t p = cl.peer(at, r < cl.size ? r : cl.rank);
+  for (int half = 0; half < kMaxCluster; half += 4) {
+    if (half >= cl.size) break;
+    u64 v[4][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[r][i] = ld_peer_u64(p + 8 * i);
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t p = cl.peer(at, half + r < cl.size ? half + r : cl.rank);
+      if constexpr (N == 1) v[r][0] = ld_peer_u64(p);
+      else
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+          asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v[r][i]), "=l"(v[r][i + 1]) : "r"(p + 8 * i) : "memory");
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f(half + r, v[r]);
   }
 }
 
@@ -220,13 +233,11 @@ __device__ __forceinline__ u64 cluster_sum(u64 v, Shared& sm, Cluster& cl, u64& 
   cl.turn ^= 1;   // the slot of the turn before may still be read
   if (threadIdx.x == 0) sm.sums[cl.turn] = mine;
   cl.sync();
-  u64 all = 0, peers[kMaxCluster][1];
-  read_peers(cl, &sm.sums[cl.turn], peers);
-#pragma unroll
-  for (int r = 0; r < kMaxCluster; ++r) {
-    before += r < cl.rank ? peers[r][0] : 0;
-    all += r < cl.size ? peers[r][0] : 0;
-  }
+  u64 all = 0;
+  read_peers<1>(cl, &sm.sums[cl.turn], [&](int r, const u64 (&v)[1]) {
+    before += r < cl.rank ? v[0] : 0;
+    all += r < cl.size ? v[0] : 0;
+  });
   return all;
 }
 
@@ -234,29 +245,21 @@ __device__ __forceinline__ u64 cluster_sum(u64 v, Shared& sm, Cluster& cl, u64& 
 __device__ __forceinline__ void cluster_bins(Shared& sm, const Cluster& cl, u64 (&x)[kPerThread]) {
   cl.sync();
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = sm.hist[kPerThread * threadIdx.x + i];
+  for (int i = 0; i < kPerThread; ++i) x[i] = cl.size == 1 ? sm.hist[kPerThread * threadIdx.x + i] : 0;
   if (cl.size == 1) return;
-  u64 v[kMaxCluster][kPerThread];
-  read_peers(cl, &sm.hist[kPerThread * threadIdx.x], v);
+  read_peers<kPerThread>(cl, &sm.hist[kPerThread * threadIdx.x], [&](int r, const u64 (&v)[kPerThread]) {
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    x[i] = 0;
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) x[i] += r < cl.size ? v[r][i] : 0;
-  }
+    for (int i = 0; i < kPerThread; ++i) x[i] += r < cl.size ? v[i] : 0;
+  });
 }
 __device__ __forceinline__ void cluster_counts(Shared& sm, const Cluster& cl, const unsigned* bins, u64 (&x)[kPerThread]) {
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = bins[kPerThread * threadIdx.x + i];
+  for (int i = 0; i < kPerThread; ++i) x[i] = cl.size == 1 ? bins[kPerThread * threadIdx.x + i] : 0;
   if (cl.size == 1) return;
-  u64 v[kMaxCluster][kPerThread / 2];
-  read_peers(cl, reinterpret_cast<const u64*>(&bins[kPerThread * threadIdx.x]), v);
+  read_peers<kPerThread / 2>(cl, reinterpret_cast<const u64*>(&bins[kPerThread * threadIdx.x]), [&](int r, const u64 (&v)[kPerThread / 2]) {
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    x[i] = 0;
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) x[i] += r < cl.size ? (v[r][i / 2] >> (32 * (i & 1))) & 0xffffffffu : 0;
-  }
+    for (int i = 0; i < kPerThread; ++i) x[i] += r < cl.size ? (v[i / 2] >> (32 * (i & 1))) & 0xffffffffu : 0;
+  });
 }
 
 // Candidates that every CTA has collected in its own list, read by the first CTA: f(candidate), each once.
@@ -270,9 +273,9 @@ __device__ __forceinline__ void pull_lists(Shared& sm, const Cluster& cl, F f) {
 }
 
 // The first index at which the running weight (vocabulary order) exceeds target_of(total weight), or -1; w(i, z) is the
-// weight of element i of the slice. The CTA that holds it divides its slice among its warps until one warp can walk it.
+// weight of element i of the slice, 0 below `floor`. The CTA that holds it divides its slice among its warps until one warp can walk it.
 template <class S, class Target, class W>
-__device__ int order_search(Shared& sm, Cluster& cl, const S& row, Target target_of, W w) {
+__device__ int order_search(Shared& sm, Cluster& cl, const S& row, float floor, long long* out, Target target_of, W w) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 s = 0, before, mine;
   // the first division is by slices of the CTAs and, inside, by sixteenths for its warps
@@ -286,6 +289,7 @@ __device__ int order_search(Shared& sm, Cluster& cl, const S& row, Target target
       u64 m[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] = row.at(i + 32 * e);
+      if (!(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) >= floor)) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) m[e] = w(i + 32 * e, z[e]);
       s += (m[0] + m[1]) + (m[2] + m[3]);
@@ -294,8 +298,10 @@ __device__ int order_search(Shared& sm, Cluster& cl, const S& row, Target target
   }
   u64 target = target_of(cluster_sum(s, sm, cl, before, mine));
   const bool here = target >= before && target - before < mine;
-  if (threadIdx.x == 0) sm.answer = -1;
-  cl.sync();
+  if (out == nullptr) {
+    if (threadIdx.x == 0) sm.answer = -1;
+    cl.sync();
+  }
   if (here) {
     target -= before;
     for (bool summed = true; hi - lo > 64; summed = false) {
@@ -332,12 +338,18 @@ __device__ int order_search(Shared& sm, Cluster& cl, const S& row, Target target
         if (over) found = i0 + __ffs(over) - 1;
         run = __shfl_sync(0xffffffffu, c, 31);
       }
-      if (lane < cl.size) {
+      if (out != nullptr) {
+        if (lane == 0) *out = row.first + found;
+      } else if (lane < cl.size) {
         const int index = found < 0 ? -1 : row.first + found;
         if (cl.size == 1) sm.answer = index;
         else st_peer_u32(cl.peer(&sm.answer, lane), static_cast<uint32_t>(index));
       }
     }
+  }
+  if (out != nullptr) {
+    if (cl.size > 1) cl.sync();   // no CTA leaves while another reads its shared memory
+    return 0;
   }
   cl.sync();
   const int r = sm.answer;
@@ -386,8 +398,7 @@ __device__ uint32_t key_search(Shared& sm, Cluster& cl, const S& row, const Expo
     cl.sync();   // the bins of the step before have been read by all
     for (int i = threadIdx.x; i < kBins; i += kThreads) sm.hist[i] = 0;
     __syncthreads();
-    row.each([&](int i, float z) {
-      if (z < ex.z_cut) return;
+    row.each(ex.z_cut, [&](int i, float z) {
       const uint32_t k = order_key(z);
       if (first) {
         if (in(i, z, k)) atomicAdd(&sm.hist[bin_of(z)], w(z));
@@ -501,11 +512,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
       sm.best[1] = static_cast<unsigned>(arg);
     }
     cl.sync();
-    u64 v[kMaxCluster][2];
-    read_peers(cl, sm.best, v);   // (this CTA's own again where the cluster is smaller)
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c)
-      take(__uint_as_float(static_cast<uint32_t>(v[c][0] >> 32)), static_cast<int>(v[c][1]), __uint_as_float(static_cast<uint32_t>(v[c][0])));
+    read_peers<2>(cl, sm.best, [&](int, const u64 (&v)[2]) {   // (this CTA's own again where the cluster is smaller)
+      take(__uint_as_float(static_cast<uint32_t>(v[0] >> 32)), static_cast<int>(v[1]), __uint_as_float(static_cast<uint32_t>(v[0])));
+    });
   }
   if (zmax == -CUDART_INF_F || !(t > 0.0f) || k == 1 || !(top_p > 0.0f) || !(min_p <= 1.0f)) {
     if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = zmax == -CUDART_INF_F ? -1 : arg;
@@ -525,14 +534,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
 
   Threshold cut;                    // what top-k and top-p keep, when the long way is taken
   cut.key = order_key(ex.z_cut);
+  float floor = ex.z_cut;           // nothing below has a mass that counts
   if (filtered) {
     const float width = fminf(zmax - zmin, kReach * t);
     const float per = width > 0.0f ? fminf(static_cast<float>(kBins) / width, 1e37f) : 0.0f;
     // the nearest whole number to (zmax - z) * per, left in the low bits by adding 2^23
     auto bin_of = [&](float z) { return min(__float_as_int(fmaf(zmax - z, per, 8388608.0f)) & 0x7fffff, kBins - 1); };
-    row.each([&](int, float z) {
-      if (z >= ex.z_cut) atomicAdd(&sm.count[bin_of(z)], 1u);
-    });
+    row.each(ex.z_cut, [&](int, float z) { atomicAdd(&sm.count[bin_of(z)], 1u); });
     cl.sync();
     u64 x[kPerThread], total;
     cluster_counts(sm, cl, sm.count, x);
@@ -549,7 +557,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
     u64 c = start;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      sm.cursor[kPerThread * threadIdx.x + i] = static_cast<unsigned>(c);
       c += x[i];
       if (static_cast<int>(kPerThread * threadIdx.x) + i == bin_cut) sm.inside = c;
     }
@@ -559,16 +566,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
     if (n_cut <= kList) {
       // ---- the short way, in the first CTA: candidates go to their bin's places, are ranked inside it, and decided on
       const float z_lo = bin_cut < kBins - 1 && per < 1e30f ? fmaxf(zmax - (bin_cut + 0.51f) / per, ex.z_cut) : ex.z_cut;
-      row.each([&](int i, float z) {
-        if (z < z_lo) return;
-        const int bin = bin_of(z);
-        if (bin > bin_cut) return;
+      row.each(z_lo, [&](int i, float z) {
+        if (bin_of(z) > bin_cut) return;
         sm.list[atomicAdd(&sm.n, 1u)] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
       });
+      if (cl.rank == 0) {
+        c = start;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) sm.count[kPerThread * threadIdx.x + i] = static_cast<unsigned>(c), c += x[i];
+      }
       cl.sync();
       if (cl.rank == 0)
         pull_lists(sm, cl, [&](u64 e) {
-          sm.sorted[atomicAdd(&sm.cursor[bin_of(key_value(static_cast<uint32_t>(e >> 32)))], 1u)] = e;
+          sm.sorted[atomicAdd(&sm.count[bin_of(key_value(static_cast<uint32_t>(e >> 32)))], 1u)] = e;
         });
       cl.sync();
       if (cl.rank != 0) return;   // nobody reads this CTA's memory any more
@@ -576,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
       for (int i = threadIdx.x; i < n; i += kThreads) {
         const u64 e = sm.sorted[i];
         const int bin = bin_of(key_value(static_cast<uint32_t>(e >> 32)));
-        const int from = bin > 0 ? sm.cursor[bin - 1] : 0, to = sm.cursor[bin];
+        const int from = bin > 0 ? sm.count[bin - 1] : 0, to = sm.count[bin];   // where the bin before, and this one, ends
         int rank = from;
         for (int j = from; j < to; ++j) rank += sm.sorted[j] > e;
         sm.list[rank] = e;
@@ -623,28 +633,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (mine[e] > 0 && index[e] / range == bucket) {
-          const unsigned at = atomicAdd(&sm.n, 1u);
-          sm.sorted[at] = index[e], sm.list_mass[at] = mine[e];
+          sm.sorted[atomicAdd(&sm.n, 1u)] = (static_cast<u64>(index[e]) << 32) | static_cast<unsigned>(N * threadIdx.x + e);
         }
       __syncthreads();
-      const int members = static_cast<int>(sm.n);
+      const int members = static_cast<int>(sm.n);   // index in the high half, place in the list in the low
+      auto mass_of = [&](u64 m) { return ex.mass(key_value(static_cast<uint32_t>(sm.list[static_cast<uint32_t>(m)] >> 32))); };
       for (int i = threadIdx.x; i < members; i += kThreads) {
         u64 cum = base;
         for (int j = 0; j < members; ++j)
-          if (sm.sorted[j] < sm.sorted[i]) cum += sm.list_mass[j];
-        if (cum <= goal && cum + sm.list_mass[i] > goal) a.out[r] = static_cast<long long>(sm.sorted[i]);
+          if (sm.sorted[j] < sm.sorted[i]) cum += mass_of(sm.sorted[j]);
+        if (cum <= goal && cum + mass_of(sm.sorted[i]) > goal) a.out[r] = static_cast<long long>(sm.sorted[i] >> 32);
       }
       return;
     }
 
     // ---- the long way: thresholds by histograms of counts and masses
+    if (bin_m < kBins - 1 && per < 1e37f) floor = fmaxf(floor, zmax - (bin_m + 0.51f) / per);   // min_p keeps nothing below
     if (above_k < static_cast<u64>(k) && total > static_cast<u64>(k)) {
       const uint32_t key = key_search(sm, cl, row, ex, bin_of, per, static_cast<double>(k), [](int, float, uint32_t) { return true; },
                                       [](float) { return 1ull; });
       const u64 ties = static_cast<u64>(k) - sm.below;   // that many of the equals are kept
       __syncthreads();
       cut.key = key;
-      cut.last = order_search(sm, cl, row, [&](u64) { return ties - 1; }, [&](int, float z) { return order_key(z) == key ? 1ull : 0ull; });
+      floor = fmaxf(floor, key_value(key));
+      cut.last = order_search(sm, cl, row, key_value(key), nullptr, [&](u64) { return ties - 1; }, [&](int, float z) { return order_key(z) == key ? 1ull : 0ull; });
       if (cut.last < 0) cut.last = 0x7fffffff;
     }
     if (nucleus) {
@@ -662,8 +674,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         cl.sync();
         for (int i = threadIdx.x; i < 3 * kBins; i += kThreads) (&sm.limb[0][0])[i] = 0;
         __syncthreads();
-        row.each([&](int i, float z) {
-          if (z < ex.z_cut) return;
+        row.each(floor, [&](int i, float z) {
           const u64 m = mass_in(i, z);
           if (m == 0) return;
           const int bin = bin_of(z);
@@ -671,15 +682,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
           atomicAdd(&sm.limb[1][bin], static_cast<unsigned>(m >> 16) & 0xffffu);
           atomicAdd(&sm.limb[2][bin], static_cast<unsigned>(m >> 32));
         });
-        cl.sync();
-        u64 y[kPerThread];
-        cluster_counts(sm, cl, sm.limb[2], x);
-        cluster_counts(sm, cl, sm.limb[1], y);
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) x[i] = (x[i] << 16) + y[i];
-        cluster_counts(sm, cl, sm.limb[0], y);
+        for (int i = 0; i < kPerThread; ++i) {   // the parts make whole masses again, in the same memory
+          const int bin = kPerThread * threadIdx.x + i;
+          x[i] = (static_cast<u64>(sm.limb[2][bin]) << 32) + (static_cast<u64>(sm.limb[1][bin]) << 16) + sm.limb[0][bin];
+        }
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) x[i] = (x[i] << 16) + y[i];
+        for (int i = 0; i < kPerThread; ++i) sm.hist[kPerThread * threadIdx.x + i] = x[i];
+        cluster_bins(sm, cl, x);
         first_reaching(sm, x, 0, [&](u64 sum) { return want = want_p * static_cast<double>(sum); }, all);
         j = sm.bin;
         const u64 above = sm.below;
@@ -689,8 +701,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
           const bool narrow = per < 1e30f;   // (bounds a hundredth of a bin wide of it)
           const float z_lo = narrow && j < kBins - 1 ? fmaxf(zmax - (j + 0.51f) / per, ex.z_cut) : ex.z_cut;
           const float z_hi = narrow && j > 0 ? zmax - (j - 0.51f) / per : zmax;
-          row.each([&](int i, float z) {
-            if (z < z_lo || z > z_hi || bin_of(z) != j || mass_in(i, z) == 0) return;
+          row.each(z_lo, [&](int i, float z) {
+            if (z > z_hi || bin_of(z) != j || mass_in(i, z) == 0) return;
             const unsigned at = atomicAdd(&sm.n, 1u);
             if (at < static_cast<unsigned>(kList))
               sm.list[at] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
@@ -698,7 +710,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
           cl.sync();
           if (cl.rank == 0) {
             u64 n_all = 0;
-            for (int c = 0; c < cl.size; ++c) n_all += ld_peer_u64(cl.peer(&sm.n, c)) & 0xffffffffu;
+            read_peers<1>(cl, reinterpret_cast<const u64*>(&sm.n),
+                          [&](int c, const u64 (&v)[1]) { n_all += c < cl.size ? v[0] & 0xffffffffu : 0; });
             const int n = static_cast<int>(n_all);
             if (threadIdx.x == 0) sm.cut_last = kNoList, sm.lo = 0;
             __syncthreads();
@@ -749,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
       if (j == -2) {
         auto in = [&](int i, float z, uint32_t) { return mass_in(i, z) > 0; };
         u64 mass = 0, b, m;
-        row.each([&](int i, float z) { mass += mass_in(i, z); });
+        row.each(floor, [&](int i, float z) { mass += mass_in(i, z); });
         all = cluster_sum(mass, sm, cl, b, m);
         want = want_p * static_cast<double>(all);
         const uint32_t key = key_search(sm, cl, row, ex, bin_of, per, want, in, [&](float z) { return ex.mass(z); });
@@ -761,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
           u64 ties = need < 1.0 ? 1 : static_cast<u64>(need);
           while (ties > 1 && static_cast<double>(above + (ties - 1) * each) >= want) --ties;
           while (static_cast<double>(above + ties * each) < want && ties < static_cast<u64>(a.vocab)) ++ties;
-          const int last = order_search(sm, cl, row, [&](u64) { return ties - 1; }, [&](int i, float z) {
+          const int last = order_search(sm, cl, row, key_value(key), nullptr, [&](u64) { return ties - 1; }, [&](int i, float z) {
             return order_key(z) == key && top.keeps(key, row.first + i) ? 1ull : 0ull;
           });
           if (last >= 0) cut.last = last;
@@ -773,18 +786,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
   }
 
   // ---- the draw, over the vocabulary
-  const int token = order_search(sm, cl, row,
-                                 [&](u64 kept) {
-                                   const u64 target = static_cast<u64>(u * static_cast<double>(kept));
-                                   return target < kept ? target : kept - 1;
-                                 },
-                                 [&](int i, float z) {
-                                   const bool keep = z >= ex.z_cut && cut.keeps(order_key(z), row.first + i);
-                                   const double p = ex.scaled(fmaxf(z, ex.z_cut));
-                                   const u64 m = Exponent::whole(p);
-                                   return keep && p >= pmin ? m : 0ull;
-                                 });
-  if (threadIdx.x == 0 && cl.rank == 0) a.out[r] = token;
+  floor = fmaxf(floor, key_value(cut.key));
+  order_search(sm, cl, row, floor, a.out + r,
+               [&](u64 kept) {
+                 const u64 target = static_cast<u64>(u * static_cast<double>(kept));
+                 return target < kept ? target : kept - 1;
+               },
+               [&](int i, float z) {
+                 const bool keep = z >= ex.z_cut && cut.keeps(order_key(z), row.first + i);
+                 const double p = ex.scaled(fmaxf(z, ex.z_cut));
+                 const u64 m = Exponent::whole(p);
+                 return keep && p >= pmin ? m : 0ull;
+               });
 }
 
 template <class T>
