@@ -37,6 +37,24 @@ constexpr int KVS = 3;     // stages of K and of V
 constexpr int kBox = 16;   // tokens per TMA box: a page holds a multiple of it
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
+// two fp32 operations per instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <int D, bool MX>
 struct ChunkLayout {
   static constexpr int kQ = BQ * D * 2;
@@ -386,9 +404,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
         }
       }
-      float m_tile = -1.0e30f;
+      float mt[4] = {-1.0e30f, -1.0e30f, -1.0e30f, -1.0e30f};   // four chains, three operands an instruction
 #pragma unroll
-      for (int e = 0; e < 64; ++e) m_tile = fmaxf(m_tile, sv[e]);
+      for (int e = 0; e < 64; e += 8)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mt[c] = fmaxf(fmaxf(mt[c], sv[e + 2 * c]), sv[e + 2 * c + 1]);
+      const float m_tile = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
       const bool raise = (m_tile - m_ref) * sl > kRescaleThreshold;
       if (__any_sync(0xffffffffu, raise)) {
         float alpha = 1.0f;
@@ -413,16 +434,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           tc_fence_before();
         }
       }
-      const float m_scaled = m_ref * sl;
+      const uint64_t sl2 = pack2(sl, sl), m2 = pack2(-m_ref * sl, -m_ref * sl);
       uint32_t packed[32];
-      float l_tile = 0.0f;
+      uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
-        const uint32_t pk = pack_bf16(fast_exp2(sv[e] * sl - m_scaled), fast_exp2(sv[e + 1] * sl - m_scaled));
-        l_tile += bf16_lo(pk) + bf16_hi(pk);
-        packed[e / 2] = pk;
+        float p0, p1;
+        unpack2(fma2(pack2(sv[e], sv[e + 1]), sl2, m2), p0, p1);
+        p0 = fast_exp2(p0), p1 = fast_exp2(p1);
+        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(p0, p1));
+        packed[e / 2] = pack_bf16(p0, p1);
       }
-      l_run += l_tile;
+      float l0, l1;
+      unpack2(add2(sum[0], sum[1]), l0, l1);
+      l_run += l0 + l1;
       tmem_st_32x32(tmem_S(x, sb) + lane_sel, packed);
       tmem_st_wait();
       tc_fence_before();
