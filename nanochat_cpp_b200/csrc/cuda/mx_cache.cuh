@@ -34,11 +34,13 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// Codes in bytes 0, 1 (lo) and 2, 3 (hi) of w -> bf16 pairs, not yet multiplied.
+// Codes in bytes 0, 1 (lo) and 2, 3 (hi) of w -> bf16 pairs, not yet multiplied. With the codes in the low bytes of 16-bit
+// fields, x * 16 puts the seven bits below the sign in place and the sign four places too low: 240 times the sign bit
+// moves it up. (Multiplications, because logic runs at half their rate and is what these loops are short of.)
 __device__ __forceinline__ void mx_spread(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t x = __byte_perm(w, 0, 0x1404), y = __byte_perm(w, 0, 0x3424);
-  lo = (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u);
-  hi = (y & 0x80008000u) | ((y >> 4) & 0x07f007f0u);
+  const uint32_t x = __byte_perm(w, 0, 0x4140), y = __byte_perm(w, 0, 0x4342);
+  lo = (x & 0x00800080u) * 240u + x * 16u;
+  hi = (y & 0x00800080u) * 240u + y * 16u;
 }
 
 }  // namespace nc
