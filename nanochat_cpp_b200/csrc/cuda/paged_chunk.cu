@@ -2,17 +2,21 @@
 //
 // Rows are (query token, head of the group): the heads that share a kv head are packed into the 128-row tiles of one CTA
 // (the largest power of two that divides the group), so keys and values are read once for all of them and a chunk
-// of a few tokens still fills a tile. A CTA takes two such tiles and walks the keys that either sees, 64 at a time:
+// of a few tokens still fills a tile. A CTA takes two such tiles and walks the keys that either sees, 128 at a time:
 //   warps 0..3, 4..7  softmax of row tile 0 and 1: a thread owns a row; P replaces S in tensor memory as bf16
-//   warp 8            tcgen05.mma: S^x = Q^x K^T (two buffers per tile), O^x += P^x V, O in tensor memory all along
+//   warp 8            tcgen05.mma: S^x = Q^x K^T, O^x += P^x V, both in tensor memory all along
 //   warp 9            TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
 //   warps 10..13      on MXFP8 pages: codes are read from global memory one tile ahead, spread to bf16, multiplied by
 //                     their block's power of two (exact) and stored in the operands' 128-byte swizzled layout
+// The products run in the order O0(j), S0(j + 1), O1(j), S1(j + 1): while one tile's softmax works, the other tile's
+// products do, and S(j + 1) needs no barrier of its own, because it follows the product that read P(j) out of its columns.
+// 128 keys at a time because a 128 x 64 product from shared memory takes 48 clocks for the 32 of its arithmetic (the
+// 128 rows of Q are read for every 64 keys), a 128 x 128 one the 64 it needs; and the waits of a step cost about 600.
 // A page that is not in the pool, and 16 tokens that no row sees, become rows of zeros; values of the first and last
 // 16 tokens that are only partly seen are copied by hand with zeros in the unseen places, because what lies there
 // (a place behind the sequence's end) may be NaN, and 0 * NaN is not 0.
 // The running maximum is raised only when a tile exceeds it by more than 2^8: then the thread rescales its O row in tensor
-// memory. Bound by the exponentials (16 a clock and SM: 512 clocks per 128 x 64 tile, against 256 for its products).
+// memory. Bounds, per 128 x 128 tile: 1024 clocks for the exponentials (16 a clock and SM), 1024 for the two products.
 // grid: (blocks of 256 rows x key runs, kv heads x head packs, sequences), the blocks that see most first.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -32,8 +36,8 @@ namespace {
 
 constexpr int BQ = 128;    // rows per tile (TMEM lanes)
 constexpr int NQ = 2;      // row tiles per CTA
-constexpr int BKV = 64;    // keys per step
-constexpr int KVS = 3;     // stages of K and of V
+constexpr int BKV = 128;   // keys per step
+constexpr int KVS = 2;     // stages of K and of V
 constexpr int kBox = 16;   // tokens per TMA box: a page holds a multiple of it
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
@@ -88,13 +92,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   uint64_t* k_empty = k_full + KVS;
   uint64_t* v_full = k_empty + KVS;
   uint64_t* v_empty = v_full + KVS;
-  uint64_t* tile_bars = v_empty + KVS;   // per row tile: s_full[2], s_empty[2], p_full[2], o_done, o_final
-  auto s_full = [&](int x, int i) { return tile_bars + 8 * x + i; };
-  auto s_empty = [&](int x, int i) { return tile_bars + 8 * x + 2 + i; };
-  auto p_full = [&](int x, int i) { return tile_bars + 8 * x + 4 + i; };
-  auto o_done = [&](int x) { return tile_bars + 8 * x + 6; };    // flips after every P V product
-  auto o_final = [&](int x) { return tile_bars + 8 * x + 7; };   // once, after the last
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tile_bars + 8 * NQ);
+  uint64_t* s_full = v_empty + KVS;      // [NQ] scores of a key tile are there
+  uint64_t* p_full = s_full + NQ;        // [NQ] its probabilities are, in their place
+  uint64_t* o_final = p_full + NQ;       // [NQ] the last P V product is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_final + NQ);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -137,13 +138,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       mbar_init(&v_empty[i], 1);
     }
     for (int x = 0; x < NQ; ++x) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(s_full(x, i), 1);
-        mbar_init(s_empty(x, i), 4);
-        mbar_init(p_full(x, i), 4);
-      }
-      mbar_init(o_done(x), 1);
-      mbar_init(o_final(x), 1);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_final[x], 1);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -165,73 +162,87 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   const bool any_bad = __syncthreads_or(bad);
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  auto tmem_S = [&](int x, int buf) { return tmem_base + x * 128 + buf * BKV; };
+  auto tmem_S = [&](int x) { return tmem_base + x * BKV; };
   auto tmem_O = [&](int x) { return tmem_base + 256 + x * 128; };
 
   if (warp == NQ * 4) {
     // ---------------------------------------------------------------- MMA issuer
     // The whole warp walks the loop and waits, one elected thread issues: control flow and descriptors stay uniform
-    // (one lane running it alone spent 40 clocks per instruction, most of a step, moving descriptors).
+    // (a single lane that ran it alone took 44 clocks to issue a product).
     constexpr uint32_t idesc_s = make_idesc_bf16(BQ, BKV, false, false);
     constexpr uint32_t idesc_o = make_idesc_bf16(BQ, D, false, true);
     const uint64_t q_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 16, 1024);
     const uint64_t k_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 16, 1024);
     const uint64_t v_desc0 = make_smem_desc_sw128(smem_u32(smem + L::kOffV), BKV * 128, 1024);
-    auto issue_s = [&](int s) -> bool {
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status, code)) != 0;
+    };
+    auto sees = [&](int x, int j) { return j >= lo[x] && j <= hi[x]; };
+    auto scores = [&](int x, int s) {          // S^x of key tile first + s
+      const uint64_t dq = q_desc0 + static_cast<uint64_t>(x * (L::kQ >> 4));
+      const uint64_t dk = k_desc0 + static_cast<uint64_t>((s % KVS) * (L::kKV >> 4));
+      const uint32_t ts = tmem_S(x);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t qo = static_cast<uint64_t>(((k / 4) * (BQ * 128) + (k % 4) * 32) >> 4);
+          const uint64_t ko = static_cast<uint64_t>(((k / 4) * (BKV * 128) + (k % 4) * 32) >> 4);
+          mma_f16_ss(ts, dq + qo, dk + ko, idesc_s, k > 0 ? 1u : 0u);
+        }
+        mma_commit(&s_full[x]);
+      }
+      __syncwarp();
+    };
+    auto free_stage = [&](uint64_t* bar) {
+      if (elect_one()) mma_commit(bar);
+      __syncwarp();
+    };
+    bool ok = wait(q_full, 0, kErrWaitFull) && wait(&k_full[0], 0, kErrWaitFull);
+    if (ok) {
+      tc_fence_after();
+      for (int x = 0; x < NQ; ++x)
+        if (sees(x, first)) scores(x, 0);
+      free_stage(&k_empty[0]);
+    }
+    for (int s = 0; s < n_u && ok; ++s) {
       const int j = first + s, st = s % KVS;
-      if (!__all_sync(0xffffffffu, mbar_wait(&k_full[st], (s / KVS) & 1, abort_flag, a.status, kErrWaitFull))) return false;
-      const uint64_t dk = k_desc0 + static_cast<uint64_t>(st * (L::kKV >> 4));
+      bool have_v = false, have_k = false;
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
-        if (j < lo[x] || j > hi[x]) continue;
-        const int i = j - lo[x];
-        if (!__all_sync(0xffffffffu, mbar_wait(s_empty(x, i & 1), ((i >> 1) & 1) ^ 1, abort_flag, a.status, kErrWaitTmemEmpty))) return false;
-        tc_fence_after();
-        const uint64_t dq = q_desc0 + static_cast<uint64_t>(x * (L::kQ >> 4));
-        const uint32_t ts = tmem_S(x, i & 1);
-        if (elect_one()) {
+        if (ok && sees(x, j)) {
+          if (!have_v) ok = wait(&v_full[st], (s / KVS) & 1, kErrWaitFull), have_v = true;
+          ok = ok && wait(&p_full[x], (j - lo[x]) & 1, kErrWaitOther);
+          if (ok) {
+            tc_fence_after();
+            const uint64_t dv = v_desc0 + static_cast<uint64_t>(st * (L::kKV >> 4));
+            const uint32_t ts = tmem_S(x), to = tmem_O(x);
+            const uint32_t more = j > lo[x] ? 1u : 0u;
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t qo = static_cast<uint64_t>(((k / 4) * (BQ * 128) + (k % 4) * 32) >> 4);
-            const uint64_t ko = static_cast<uint64_t>(((k / 4) * (BKV * 128) + (k % 4) * 32) >> 4);
-            mma_f16_ss(ts, dq + qo, dk + ko, idesc_s, k > 0 ? 1u : 0u);
+              for (int k = 0; k < BKV / 16; ++k)   // P of 64 keys takes the first 32 of their 64 score columns
+                mma_f16_ts(to, ts + (k / 4) * 64 + (k % 4) * 8, dv + static_cast<uint64_t>((k * 16 * 128) >> 4), idesc_o,
+                           k > 0 ? 1u : more);
+              if (j == hi[x]) mma_commit(&o_final[x]);
+            }
+            __syncwarp();
           }
-          mma_commit(s_full(x, i & 1));
         }
-        __syncwarp();
-      }
-      if (elect_one()) mma_commit(&k_empty[st]);
-      __syncwarp();
-      return true;
-    };
-    auto issue_o = [&](int s) -> bool {
-      const int j = first + s, st = s % KVS;
-      if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (s / KVS) & 1, abort_flag, a.status, kErrWaitFull))) return false;
-      const uint64_t dv = v_desc0 + static_cast<uint64_t>(st * (L::kKV >> 4));
-#pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        if (j < lo[x] || j > hi[x]) continue;
-        const int i = j - lo[x];
-        if (!__all_sync(0xffffffffu, mbar_wait(p_full(x, i & 1), (i >> 1) & 1, abort_flag, a.status, kErrWaitOther))) return false;
-        tc_fence_after();
-        const uint32_t ts = tmem_S(x, i & 1);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < BKV / 16; ++k)
-            mma_f16_ts(tmem_O(x), ts + k * 8, dv + static_cast<uint64_t>((k * 16 * 128) >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
-          mma_commit(o_done(x));
-          if (j == hi[x]) mma_commit(o_final(x));
+        if (ok && s + 1 < n_u && sees(x, j + 1)) {
+          if (!have_k) ok = wait(&k_full[(s + 1) % KVS], ((s + 1) / KVS) & 1, kErrWaitFull), have_k = true;
+          if (ok) {
+            tc_fence_after();
+            scores(x, s + 1);
+          }
         }
-        __syncwarp();
       }
-      if (elect_one()) mma_commit(&v_empty[st]);
-      __syncwarp();
-      return true;
-    };
-    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, a.status, kErrWaitFull));
-    for (int s = 0; s <= n_u && ok; ++s) {
-      if (s < n_u) ok = issue_s(s);
-      if (ok && s >= 1) ok = issue_o(s - 1);
+      if (ok) {
+        if (!have_v) ok = wait(&v_full[st], (s / KVS) & 1, kErrWaitFull);   // a tile that neither row tile sees
+        if (ok && s + 1 < n_u && !have_k) ok = wait(&k_full[(s + 1) % KVS], ((s + 1) / KVS) & 1, kErrWaitFull);
+        if (ok) {
+          free_stage(&v_empty[st]);
+          if (s + 1 < n_u) free_stage(&k_empty[(s + 1) % KVS]);
+        }
+      }
     }
   } else if (warp == NQ * 4 + 1) {
     // ---------------------------------------------------------------- TMA: Q, and bf16 keys and values
@@ -249,8 +260,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       int st = 0;
       uint32_t ph = 0;
       for (int s = 0; s < n_u && ok; ++s) {
-        // lanes 0..3: the four boxes of the tile
-        const int key = (first + s) * BKV + (lane & 3) * kBox;
+        // lanes 0..7: the boxes of the tile
+        const int key = (first + s) * BKV + (lane & 7) * kBox;
         int row = out_of_pool;
         bool partial = false;
         if (key + kBox > rg.lo && key < rg.hi) {
@@ -258,14 +269,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           if (page >= 0 && page < a.num_pages) row = page * a.page_size + key % a.page_size;
           partial = row != out_of_pool && (key < rg.lo || key + kBox > rg.hi);
         }
-        const unsigned by_hand = __ballot_sync(0xffffffffu, partial && lane < 4);
+        const unsigned by_hand = __ballot_sync(0xffffffffu, partial && lane < BKV / kBox);
         ok = mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         uint8_t* sk = smem + L::kOffK + st * L::kKV;
         uint8_t* sv = smem + L::kOffV + st * L::kKV;
         if (lane == 0) mbar_expect_tx(&k_full[st], L::kKV);
         __syncwarp();
-        if (lane < 4)
+        if (lane < BKV / kBox)
 #pragma unroll
           for (int c = 0; c < DC; ++c)
             tma_load_3d(sk + c * (BKV * 128) + lane * (kBox * 128), &tmK, &k_full[st], c * 64, row, kvh);
@@ -273,7 +284,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         ok = mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         if (by_hand != 0) {
-          for (int box = 0; box < 4; ++box) {
+          for (int box = 0; box < BKV / kBox; ++box) {
             if (((by_hand >> box) & 1) == 0) continue;
             const int row_b = __shfl_sync(0xffffffffu, row, box), key_b = (first + s) * BKV + box * kBox;
             const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.v_pool) +
@@ -291,7 +302,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         if (lane == 0) mbar_expect_tx(&v_full[st], L::kKV - __popc(by_hand) * kBox * D * 2);
         __syncwarp();
-        if (lane < 4 && !partial)
+        if (lane < BKV / kBox && !partial)
 #pragma unroll
           for (int c = 0; c < DC; ++c)
             tma_load_3d(sv + c * (BKV * 128) + lane * (kBox * 128), &tmV, &v_full[st], c * 64, row, kvh);
@@ -317,10 +328,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const uint8_t *ksp = a.k_scale + s_off, *vsp = a.v_scale + s_off;
       uint4 kc[N], vc[N];
       uint32_t kb[N], vb[N];
-      // lanes 0..3 look up the pages of a tile's four boxes (as page * page_size + slot and page), one tile ahead of its codes
+      // lanes 0..7 look up the pages of a tile's eight boxes (as page * page_size + slot and page), one tile ahead of its codes
       int look_row = -1, look_page = -1;
       auto look = [&](int s) {
-        const int key = (first + s) * BKV + (lane & 3) * kBox;
+        const int key = (first + s) * BKV + (lane & 7) * kBox;
         look_row = look_page = -1;
         if (s < n_u && key + kBox > rg.lo && key < rg.hi) {
           const int lp = key / a.page_size, page = table[lp];
@@ -405,29 +416,26 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const float sl = a.scale * 1.4426950408889634f;
     float m_ref = -1.0e30f, l_run = 0.0f;
     bool ok = true;
+    float sv[64];
     for (int i = 0; i < n_x && ok; ++i) {
-      const int sb = i & 1;
       const int kv0 = (lo[x] + i) * BKV;
       const bool need_mask = any_bad || kv0 + BKV - 1 > pos_min || (a.window_left >= 0 && kv0 < pos_max - a.window_left) || kv0 + BKV > rg.hi;
-      if (!mbar_wait(s_full(x, sb), (i >> 1) & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t r0v[32], r1v[32];
-      tmem_ld_32x32(tmem_S(x, sb) + lane_sel, r0v);
-      tmem_ld_32x32(tmem_S(x, sb) + 32 + lane_sel, r1v);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty(x, sb));
-      float sv[64];
+      // scores of 64 keys, unseen ones -infinity: the maximum wants all 128 first, so the first half is read twice
+      auto load = [&](int half) {
+        uint32_t r0v[32], r1v[32];
+        tmem_ld_32x32(tmem_S(x) + half * 64 + lane_sel, r0v);
+        tmem_ld_32x32(tmem_S(x) + half * 64 + 32 + lane_sel, r1v);
+        tmem_ld_wait();
 #pragma unroll
-      for (int e = 0; e < 32; ++e) sv[e] = __uint_as_float(r0v[e]), sv[32 + e] = __uint_as_float(r1v[e]);
-      if (need_mask) {
-        // keys [k_lo, k_hi) of this tile are seen by the row; the rest cannot be told from seen ones by value
-        const int k_hi = min(qpos + 1, rg.hi) - kv0, k_lo = (a.window_left >= 0 ? max(0, qpos - a.window_left) : 0) - kv0;
+        for (int e = 0; e < 32; ++e) sv[e] = __uint_as_float(r0v[e]), sv[32 + e] = __uint_as_float(r1v[e]);
+        if (!need_mask) return;
+        // keys [k_lo, k_hi) of the half are seen by the row; the rest cannot be told from seen ones by value
+        const int k0 = kv0 + half * 64;
+        const int k_hi = min(qpos + 1, rg.hi) - k0, k_lo = (a.window_left >= 0 ? max(0, qpos - a.window_left) : 0) - k0;
 #pragma unroll
         for (int e = 0; e < 64; ++e) sv[e] = e >= k_lo && e < k_hi ? sv[e] : -CUDART_INF_F;
-        for (int box = 0; any_bad && box < BKV / kBox; ++box) {   // a page outside the pool: its keys are none
-          const int key = kv0 + box * kBox;
+        for (int box = 0; any_bad && box < 64 / kBox; ++box) {   // a page outside the pool: its keys are none
+          const int key = k0 + box * kBox;
           if (key >= rg.hi || key + kBox <= rg.lo) continue;
           const int page = table[key / a.page_size];
           if (page < 0 || page >= a.num_pages) {
@@ -435,13 +443,38 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int e = 0; e < 64; ++e) sv[e] = (e >> 4) == box ? -CUDART_INF_F : sv[e];
           }
         }
-      }
-      float mt[4] = {-1.0e30f, -1.0e30f, -1.0e30f, -1.0e30f};   // four chains, three operands an instruction
+      };
+      auto largest = [&](float m) {
+        float mt[4] = {m, m, m, m};   // four chains, three operands an instruction
 #pragma unroll
-      for (int e = 0; e < 64; e += 8)
+        for (int e = 0; e < 64; e += 8)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mt[c] = fmaxf(fmaxf(mt[c], sv[e + 2 * c]), sv[e + 2 * c + 1]);
-      const float m_tile = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
+          for (int c = 0; c < 4; ++c) mt[c] = fmaxf(fmaxf(mt[c], sv[e + 2 * c]), sv[e + 2 * c + 1]);
+        return fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
+      };
+      auto probabilities = [&](int half) {
+        const uint64_t sl2 = pack2(sl, sl), m2 = pack2(-m_ref * sl, -m_ref * sl);
+        uint32_t packed[32];
+        uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          float p0, p1;
+          unpack2(fma2(pack2(sv[e], sv[e + 1]), sl2, m2), p0, p1);
+          p0 = fast_exp2(p0), p1 = fast_exp2(p1);
+          sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(p0, p1));
+          packed[e / 2] = pack_bf16(p0, p1);
+        }
+        float l0, l1;
+        unpack2(add2(sum[0], sum[1]), l0, l1);
+        l_run += l0 + l1;
+        tmem_st_32x32(tmem_S(x) + half * 64 + lane_sel, packed);
+      };
+      if (!mbar_wait(&s_full[x], i & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
+      tc_fence_after();
+      load(0);
+      float m_tile = largest(-1.0e30f);
+      load(1);
+      m_tile = largest(m_tile);
       const bool raise = (m_tile - m_ref) * sl > kRescaleThreshold;
       if (__any_sync(0xffffffffu, raise)) {
         float alpha = 1.0f;
@@ -450,9 +483,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           m_ref = m_tile;
           l_run *= alpha;
         }
-        if (i > 0) {
-          if (!mbar_wait(o_done(x), (i - 1) & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
-          tc_fence_after();
+        if (i > 0) {   // the scores of this tile came after the P V product of the one before: O is at rest
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -462,31 +493,17 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             tmem_st_32x16(tmem_O(x) + c * 16 + lane_sel, o);
           }
-          tmem_st_wait();
-          tc_fence_before();
         }
       }
-      const uint64_t sl2 = pack2(sl, sl), m2 = pack2(-m_ref * sl, -m_ref * sl);
-      uint32_t packed[32];
-      uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-#pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        float p0, p1;
-        unpack2(fma2(pack2(sv[e], sv[e + 1]), sl2, m2), p0, p1);
-        p0 = fast_exp2(p0), p1 = fast_exp2(p1);
-        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(p0, p1));
-        packed[e / 2] = pack_bf16(p0, p1);
-      }
-      float l0, l1;
-      unpack2(add2(sum[0], sum[1]), l0, l1);
-      l_run += l0 + l1;
-      tmem_st_32x32(tmem_S(x, sb) + lane_sel, packed);
+      probabilities(1);
+      load(0);
+      probabilities(0);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(x, sb));
+      if (lane == 0) mbar_arrive(&p_full[x]);
     }
-    if (ok && n_x > 0) ok = mbar_wait(o_final(x), 0, abort_flag, a.status, kErrWaitTmemFull);
+    if (ok && n_x > 0) ok = mbar_wait(&o_final[x], 0, abort_flag, a.status, kErrWaitTmemFull);
     if (ok) {
       tc_fence_after();
       const bool any = n_x > 0;                 // else O was never written
