@@ -6,8 +6,8 @@
 //   warps 0..3, 4..7  softmax of row tile 0 and 1: a thread owns a row; P replaces S in tensor memory as bf16
 //   warp 8            tcgen05.mma: S^x = Q^x K^T, O^x += P^x V, both in tensor memory all along
 //   warp 9            TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
-//   warps 10..13      on MXFP8 pages: codes are read from global memory one tile ahead, spread to bf16, multiplied by
-//                     their block's power of two (exact) and stored in the operands' 128-byte swizzled layout
+//   warps 10..13      on MXFP8 pages: codes are copied (cp.async) one tile ahead, spread to bf16, multiplied by their
+//                     block's power of two (exact) and stored in the operands' 128-byte swizzled layout
 // The products run in the order O0(j), S0(j + 1), O1(j), S1(j + 1): while one tile's softmax works, the other tile's
 // products do, and S(j + 1) needs no barrier of its own, because it follows the product that read P(j) out of its columns.
 // 128 keys at a time because a 128 x 64 product from shared memory takes 48 clocks for the 32 of its arithmetic (the
@@ -66,7 +66,10 @@ struct ChunkLayout {
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + NQ * kQ;
   static constexpr int kOffV = kOffK + KVS * kKV;
-  static constexpr int kOffBar = kOffV + KVS * kKV;
+  static constexpr int kRaw = MX ? BKV * D : 0;                // codes of a tile, one side, as they lie in memory
+  static constexpr int kOffRaw = kOffV + KVS * kKV;            // K, V
+  static constexpr int kOffScale = kOffRaw + 2 * kRaw;         // scale bytes [BKV][D / 32], K, V
+  static constexpr int kOffBar = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);
   static constexpr int kTotal = kOffBar + 512 + 1024;
   static constexpr int kThreads = (NQ * 4 + 2 + (MX ? 4 : 0)) * 32;
 };
@@ -324,56 +327,71 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const uint32_t stride = static_cast<uint32_t>(p.KV) * D, s_stride = static_cast<uint32_t>(p.KV) * a.page_size * (D / 32);
       const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
       const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
-      const long long s_off = (static_cast<long long>(kvh) * a.page_size + in_box) * (D / 32) + u / 2;
+      const long long s_off = (static_cast<long long>(kvh) * a.page_size + in_box) * (D / 32);
       const uint8_t *ksp = a.k_scale + s_off, *vsp = a.v_scale + s_off;
-      uint4 kc[N], vc[N];
-      uint32_t kb[N], vb[N];
-      // lanes 0..7 look up the pages of a tile's eight boxes (as page * page_size + slot and page), one tile ahead of its codes
-      int look_row = -1, look_page = -1;
+      const uint32_t raw = smem_u32(smem + L::kOffRaw) + t * 16, scale_at = smem_u32(smem + L::kOffScale);
+      // Lanes 0..7 look up the pages of a tile's eight boxes, two tiles ahead of its codes: the number is asked for here and
+      // looked at in `settle`, a tile later. Slot of a box in its page: the same for all tiles but for the page's turn.
+      int next_id = -1, next_slot = 0, page_l = -1, slot_l = 0;
+      bool plain = false;   // every row of the tile is wanted and every page is one of the pool's
       auto look = [&](int s) {
         const int key = (first + s) * BKV + (lane & 7) * kBox;
-        look_row = look_page = -1;
+        next_id = -1, next_slot = 0;
         if (s < n_u && key + kBox > rg.lo && key < rg.hi) {
-          const int lp = key / a.page_size, page = table[lp];
-          if (page >= 0 && page < a.num_pages) look_page = page, look_row = key - lp * a.page_size;
+          const int lp = key / a.page_size;
+          next_slot = key - lp * a.page_size;
+          next_id = table[lp];
         }
       };
-      auto fetch = [&](int s) {
-        const int key0 = (first + s) * BKV;
-        const bool inside = key0 >= rg.lo && key0 + BKV <= rg.hi;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int box = box0 + i * kBoxStep;
-          const int page = __shfl_sync(0xffffffffu, look_page, box), slot = __shfl_sync(0xffffffffu, look_row, box);
-          const int key = key0 + row0 + i * kRows;
-          kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
-          kb[i] = vb[i] = 127;
-          if (page >= 0 && (inside || (key >= rg.lo && key < rg.hi))) {
-            const unsigned long long at = static_cast<unsigned long long>(static_cast<unsigned>(page) * static_cast<unsigned>(a.page_size) + slot) * stride;
-            const unsigned long long sc = static_cast<unsigned long long>(static_cast<unsigned>(page)) * s_stride + slot * (D / 32);
-            kc[i] = *reinterpret_cast<const uint4*>(kp + at);
-            vc[i] = *reinterpret_cast<const uint4*>(vp + at);
-            kb[i] = ksp[sc];
-            vb[i] = vsp[sc];
+      auto settle = [&](int s) {
+        page_l = next_id >= 0 && next_id < a.num_pages ? next_id : -1, slot_l = next_slot;
+        plain = (first + s) * BKV >= rg.lo && (first + s + 1) * BKV <= rg.hi && __all_sync(0xffffffffu, page_l >= 0);
+      };
+      // A thread copies the pieces that it will convert; rows and pages that are not wanted arrive as zeros. The scale bytes of
+      // a row (or of two, where they are two each: a copy takes four) come with its first piece, for the whole warp.
+      auto fetch = [&](int s, int side, const uint8_t* codes, const uint8_t* scales) {
+        if (s < n_u) {
+#pragma unroll 4
+          for (int i = 0; i < N; ++i) {
+            const int box = box0 + i * kBoxStep, r = row0 + i * kRows, key = (first + s) * BKV + r;
+            const int id = __shfl_sync(0xffffffffu, page_l, box), slot = __shfl_sync(0xffffffffu, slot_l, box);
+            const bool ok = plain || (id >= 0 && key >= rg.lo && key < rg.hi);
+            const bool two = D == 64 && (plain || (ok && key + 1 < rg.hi));
+            const unsigned page = id >= 0 ? id : 0;
+            const uint8_t* c = codes + static_cast<unsigned long long>(page * static_cast<unsigned>(a.page_size) + slot) * stride;
+            const uint8_t* sc = scales + static_cast<unsigned long long>(page) * s_stride + slot * (D / 32);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + side * L::kRaw + i * 2048), "l"(c), "r"(ok ? 16 : 0) : "memory");
+            if (u == 0 && (D == 128 || (r & 1) == 0))
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scale_at + (side * BKV + r) * (D / 32)), "l"(sc),
+                           "r"(D == 128 ? (ok ? 4 : 0) : (two || (id >= 0 && key + 1 >= rg.lo && key + 1 < rg.hi) ? 4 : ok ? 2 : 0))
+                           : "memory");
           }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      auto store = [&](uint8_t* base, const uint4 (&code)[N], const uint32_t (&sb)[N]) {
-#pragma unroll
+      auto store = [&](uint8_t* base, int side) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+#pragma unroll 2
         for (int i = 0; i < N; ++i) {
           const int r = row0 + i * kRows;
-          const uint32_t f1 = mx_factor_first(sb[i]) * 0x10001u;
-          const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+          uint4 code;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w)
+                       : "r"(raw + side * L::kRaw + i * 2048) : "memory");
+          const uint32_t sb = smem[L::kOffScale + (side * BKV + r) * (D / 32) + u / 2];
+          const uint32_t f1 = mx_factor_first(sb) * 0x10001u;
+          const uint32_t w[4] = {code.x, code.y, code.z, code.w};
           uint32_t o[8];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             mx_spread(w[y], o[2 * y], o[2 * y + 1]);
             o[2 * y] = mul_bf16x2(o[2 * y], f1), o[2 * y + 1] = mul_bf16x2(o[2 * y + 1], f1);
           }
-          if (sb[i] > 134u) {
-            const uint32_t f2 = mx_factor_second(sb[i]) * 0x10001u;
+          if (sb > 134u) {
+            const uint32_t f2 = mx_factor_second(sb) * 0x10001u;
+            const bool zero = (code.x | code.y | code.z | code.w) == 0;   // rows that are none, beside scales that may be anything
 #pragma unroll
-            for (int y = 0; y < 8; ++y) o[y] = mul_bf16x2(o[y], f2);
+            for (int y = 0; y < 8; ++y) o[y] = zero ? 0u : mul_bf16x2(o[y], f2);
           }
           uint8_t* row = base + (u >> 2) * (BKV * 128) + r * 128;
           const int g = (u & 3) * 2;
@@ -385,22 +403,26 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       };
       int st = 0;
       uint32_t ph = 0;
+      // each side's next codes are requested as soon as its staging area is free, and arrive while the other side is stored
       look(0);
-      fetch(0);
+      settle(0);
+      fetch(0, 0, kp, ksp);
+      fetch(0, 1, vp, vsp);
       look(1);
       for (int s = 0; s < n_u; ++s) {
         if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty))) break;
-        store(smem + L::kOffK + st * L::kKV, kc, kb);
+        store(smem + L::kOffK + st * L::kKV, 0);
         if (lane == 0) mbar_arrive(&k_full[st]);
+        settle(s + 1);
+        fetch(s + 1, 0, kp, ksp);
+        look(s + 2);
         if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty))) break;
-        store(smem + L::kOffV + st * L::kKV, vc, vb);
+        store(smem + L::kOffV + st * L::kKV, 1);
         if (lane == 0) mbar_arrive(&v_full[st]);
-        if (s + 1 < n_u) {
-          fetch(s + 1);
-          look(s + 2);
-        }
+        fetch(s + 1, 1, vp, vsp);
         if (++st == KVS) { st = 0; ph ^= 1; }
       }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
   } else {
     // ---------------------------------------------------------------- softmax

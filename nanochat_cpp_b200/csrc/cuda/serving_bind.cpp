@@ -30,7 +30,7 @@ void check_pools(const char* op, const Tensor& k, const Tensor& v, const OptTens
   TORCH_CHECK(v.sizes() == k.sizes(), op, ": v_pool must have the shape of k_pool");
   same_device(v, k, op, "v_pool");
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, op, ": head_dim must be 64 or 128");
-  TORCH_CHECK(k.size(0) < (1LL << 31) && k.size(1) > 0 && k.size(1) < (1 << 20) && k.size(2) > 0, op, ": pool sizes out of range");
+  TORCH_CHECK(k.size(0) > 0 && k.size(0) < (1LL << 31) && k.size(1) > 0 && k.size(1) < (1 << 20) && k.size(2) > 0, op, ": pool sizes out of range");
   if (!mx) return;
   for (const OptTensor* s : {&ks, &vs}) {
     TORCH_CHECK((*s)->scalar_type() == torch::kUInt8 && (*s)->dim() == 4 && (*s)->is_contiguous() && aligned16(**s) &&

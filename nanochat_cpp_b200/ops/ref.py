@@ -627,7 +627,7 @@ def _check_mx_pools(name, k_pool, v_pool, k_scale, v_scale):
            f"{name}: v_pool must have the shape and type of k_pool")
     P, page, KV, D = k_pool.shape
     _check(D in (64, 128), f"{name}: head_dim must be 64 or 128")
-    _check(page > 0 and KV > 0, f"{name}: page_size and kv heads must be positive")
+    _check(P > 0 and page > 0 and KV > 0, f"{name}: pages, page_size and kv heads must be positive")
     for s in (k_scale, v_scale):
         _check(s is not None and s.dtype == torch.uint8 and tuple(s.shape) == (P, KV, page, D // 32) and s.is_contiguous(),
                f"{name}: scales must be contiguous uint8 [pages, KV, page_size, D / 32]")
@@ -761,7 +761,8 @@ def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, 
         _check(k_pool.dim() == 4 and k_pool.dtype == q.dtype and k_pool.is_contiguous() and v_pool.shape == k_pool.shape and
                v_pool.dtype == q.dtype and v_pool.is_contiguous(),
                f"{name}: pools must be contiguous [pages, page_size, KV, D] of q's type")
-    _check(k_pool.shape[3] == D and H % k_pool.shape[2] == 0, f"{name}: heads must be a multiple of kv heads, one head_dim")
+    _check(k_pool.shape[0] > 0 and k_pool.shape[1] > 0, f"{name}: the pools must hold pages")
+    _check(k_pool.shape[3] == D and k_pool.shape[2] > 0 and H % k_pool.shape[2] == 0, f"{name}: heads must be a multiple of kv heads, one head_dim")
     _check_table(name, page_table, B)
     for x in (seq_lens, q_lens):
         _check(x is None or (x.dtype == torch.int32 and tuple(x.shape) == (B,) and x.is_contiguous()),
