@@ -6,7 +6,7 @@
 //   warps 0..3, 4..7  softmax of row tile 0 and 1: a thread owns a row; P replaces S in tensor memory as bf16
 //   warp 8            tcgen05.mma: S^x = Q^x K^T, O^x += P^x V, both in tensor memory all along
 //   warp 9            TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
-//   warps 10..13      on MXFP8 pages: codes are copied (cp.async) one tile ahead, spread to bf16, multiplied by their
+//   warps 10..13 (K), 14..17 (V)  on MXFP8 pages: codes are copied (cp.async) one tile ahead, spread to bf16, multiplied by their
 //                     block's power of two (exact) and stored in the operands' 128-byte swizzled layout
 // The products run in the order O0(j), S0(j + 1), O1(j), S1(j + 1): while one tile's softmax works, the other tile's
 // products do, and S(j + 1) needs no barrier of its own, because it follows the product that read P(j) out of its columns.
@@ -71,7 +71,7 @@ struct ChunkLayout {
   static constexpr int kOffScale = kOffRaw + 2 * kRaw;         // scale bytes [BKV][D / 32], K, V
   static constexpr int kOffBar = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);
   static constexpr int kTotal = kOffBar + 512 + 1024;
-  static constexpr int kThreads = (NQ * 4 + 2 + (MX ? 4 : 0)) * 32;
+  static constexpr int kThreads = (NQ * 4 + 2 + (MX ? 8 : 0)) * 32;
 };
 
 struct ChunkParams {
@@ -322,14 +322,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       constexpr int U = D / 16;                 // 16-code pieces of a row
       constexpr int N = BKV * U / 128;          // pieces per thread and side: rows t / U + i * (128 / U)
       constexpr int kRows = 128 / U, kBoxStep = kRows / kBox;
-      const int t = threadIdx.x - (NQ * 4 + 2) * 32;
+      const int side = (warp - (NQ * 4 + 2)) >> 2;   // 0: keys, 1: values
+      const int t = (threadIdx.x - (NQ * 4 + 2) * 32) & 127;
       const int row0 = t / U, u = t % U, in_box = row0 % kBox, box0 = row0 / kBox;
       const uint32_t stride = static_cast<uint32_t>(p.KV) * D, s_stride = static_cast<uint32_t>(p.KV) * a.page_size * (D / 32);
-      const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
-      const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
-      const long long s_off = (static_cast<long long>(kvh) * a.page_size + in_box) * (D / 32);
-      const uint8_t *ksp = a.k_scale + s_off, *vsp = a.v_scale + s_off;
-      const uint32_t raw = smem_u32(smem + L::kOffRaw) + t * 16, scale_at = smem_u32(smem + L::kOffScale);
+      const uint8_t* codes = static_cast<const uint8_t*>(side ? a.v_pool : a.k_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
+      const uint8_t* scales = (side ? a.v_scale : a.k_scale) + (static_cast<long long>(kvh) * a.page_size + in_box) * (D / 32);
+      const uint32_t raw = smem_u32(smem + L::kOffRaw) + side * L::kRaw + t * 16;
+      uint8_t* const scale_sm = smem + L::kOffScale + side * BKV * (D / 32);
+      const uint32_t scale_at = smem_u32(scale_sm);
+      uint64_t *full = side ? v_full : k_full, *empty = side ? v_empty : k_empty;
       // Lanes 0..7 look up the pages of a tile's eight boxes, two tiles ahead of its codes: the number is asked for here and
       // looked at in `settle`, a tile later. Slot of a box in its page: the same for all tiles but for the page's turn.
       int next_id = -1, next_slot = 0, page_l = -1, slot_l = 0;
@@ -349,7 +351,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       };
       // A thread copies the pieces that it will convert; rows and pages that are not wanted arrive as zeros. The scale bytes of
       // a row (or of two, where they are two each: a copy takes four) come with its first piece, for the whole warp.
-      auto fetch = [&](int s, int side, const uint8_t* codes, const uint8_t* scales) {
+      auto fetch = [&](int s) {
         if (s < n_u) {
 #pragma unroll 4
           for (int i = 0; i < N; ++i) {
@@ -360,25 +362,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const unsigned page = id >= 0 ? id : 0;
             const uint8_t* c = codes + static_cast<unsigned long long>(page * static_cast<unsigned>(a.page_size) + slot) * stride;
             const uint8_t* sc = scales + static_cast<unsigned long long>(page) * s_stride + slot * (D / 32);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + side * L::kRaw + i * 2048), "l"(c), "r"(ok ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + i * 2048), "l"(c), "r"(ok ? 16 : 0) : "memory");
             if (u == 0 && (D == 128 || (r & 1) == 0))
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scale_at + (side * BKV + r) * (D / 32)), "l"(sc),
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scale_at + r * (D / 32)), "l"(sc),
                            "r"(D == 128 ? (ok ? 4 : 0) : (two || (id >= 0 && key + 1 >= rg.lo && key + 1 < rg.hi) ? 4 : ok ? 2 : 0))
                            : "memory");
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      auto store = [&](uint8_t* base, int side) {
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      auto store = [&](uint8_t* base) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();
-#pragma unroll 2
+#pragma unroll 4
         for (int i = 0; i < N; ++i) {
           const int r = row0 + i * kRows;
           uint4 code;
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w)
-                       : "r"(raw + side * L::kRaw + i * 2048) : "memory");
-          const uint32_t sb = smem[L::kOffScale + (side * BKV + r) * (D / 32) + u / 2];
+                       : "r"(raw + i * 2048) : "memory");
+          const uint32_t sb = scale_sm[r * (D / 32) + u / 2];
           const uint32_t f1 = mx_factor_first(sb) * 0x10001u;
           const uint32_t w[4] = {code.x, code.y, code.z, code.w};
           uint32_t o[8];
@@ -403,23 +405,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       };
       int st = 0;
       uint32_t ph = 0;
-      // each side's next codes are requested as soon as its staging area is free, and arrive while the other side is stored
+      // the next codes are requested as soon as the staging area is free, and arrive while this warp waits for a stage
       look(0);
       settle(0);
-      fetch(0, 0, kp, ksp);
-      fetch(0, 1, vp, vsp);
+      fetch(0);
       look(1);
       for (int s = 0; s < n_u; ++s) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty))) break;
-        store(smem + L::kOffK + st * L::kKV, 0);
-        if (lane == 0) mbar_arrive(&k_full[st]);
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty))) break;
+        store(smem + (side ? L::kOffV : L::kOffK) + st * L::kKV);
+        if (lane == 0) mbar_arrive(&full[st]);
         settle(s + 1);
-        fetch(s + 1, 0, kp, ksp);
+        fetch(s + 1);
         look(s + 2);
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, kErrWaitEmpty))) break;
-        store(smem + L::kOffV + st * L::kKV, 1);
-        if (lane == 0) mbar_arrive(&v_full[st]);
-        fetch(s + 1, 1, vp, vsp);
         if (++st == KVS) { st = 0; ph ^= 1; }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
