@@ -652,12 +652,19 @@ PagedPlan paged_chunk_plan(const PagedAttnArgs& a) {
   return p;
 }
 
-bool paged_chunk_takes(const PagedAttnArgs& a) {
-  // Few rows per kv head leave most of a 128-row tile empty: the other kernel reads the keys at full speed. TMA boxes
-  // are 16 tokens of one page. A scale that is not positive turns the maximum around.
-  const int P = pack_of(a.H / a.KV);
-  return a.T * (a.H / a.KV) > 16 && a.page_size % kBox == 0 && a.scale > 0.0f && a.H / P <= 65535 &&
+bool paged_chunk_can(const PagedAttnArgs& a) {
+  // TMA boxes are 16 tokens of one page. A scale that is not positive turns the maximum around.
+  return a.page_size % kBox == 0 && a.scale > 0.0f && a.H / pack_of(a.H / a.KV) <= 65535 &&
          static_cast<long long>(a.num_pages) * a.page_size < (1LL << 31) - 1024;
+}
+
+bool paged_chunk_takes(const PagedAttnArgs& a) {
+  // Few rows per kv head leave most of a 128-row tile empty, and the other kernel reads the keys at full speed. Little work
+  // in all is done before this kernel has started up: up to some 1.5 GFLOP (as many as the page table has room for) the
+  // other is faster (3 x 77 tokens, 4 heads of 64, 777 keys: 14 against 25 us).
+  double keys = static_cast<double>(a.max_pages) * a.page_size;
+  if (a.window_left >= 0) keys = std::min(keys, static_cast<double>(a.window_left) + 1 + a.T);
+  return a.T * (a.H / a.KV) > 16 && 4.0 * a.D * a.H * a.T * a.B * keys > 1.5e9 && paged_chunk_can(a);
 }
 
 const char* paged_chunk_attention(const PagedAttnArgs& a, cudaStream_t s) {

@@ -55,7 +55,8 @@ struct PagedPlan {
 };
 PagedPlan paged_rows_plan(const PagedAttnArgs& a);
 const char* paged_rows_attention(const PagedAttnArgs& a, cudaStream_t s);
-// The same for many rows per kv head (`paged_chunk_takes`: sizes it is meant for and can do).
+// The same for many rows per kv head: whether it can take these arguments, and whether it is the faster one for them.
+bool paged_chunk_can(const PagedAttnArgs& a);
 bool paged_chunk_takes(const PagedAttnArgs& a);
 PagedPlan paged_chunk_plan(const PagedAttnArgs& a);
 const char* paged_chunk_attention(const PagedAttnArgs& a, cudaStream_t s);

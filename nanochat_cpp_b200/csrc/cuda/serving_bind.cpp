@@ -112,7 +112,7 @@ std::vector<Tensor> kv_read_mx(const Tensor& k_pool, const Tensor& v_pool, const
 // q [B, T, H, D] (any strides that are multiples of 8); the result is dense and of q's shape.
 Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool, const Tensor& v_pool, const Tensor& page_table,
                        const Tensor& seq_lens, const OptTensor& q_lens, int64_t window_left, double scale,
-                       const OptTensor& k_scale, const OptTensor& v_scale) {
+                       const OptTensor& k_scale, const OptTensor& v_scale, int64_t variant) {
   const c10::cuda::CUDAGuard g(k_pool.device());
   check_pools(op, k_pool, v_pool, k_scale, v_scale);
   same_device(q_in, k_pool, op, "q");
@@ -144,7 +144,9 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   a.scale = static_cast<float>(scale);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.status = ncbind::device_status(k_pool.get_device());
-  const bool chunk = nc::paged_chunk_takes(a);
+  TORCH_CHECK(variant >= 0 && variant <= 2 && (variant != 2 || nc::paged_chunk_can(a)), op,
+              ": variant must be 0 (by size), 1 (few rows) or 2 (many rows: page_size a multiple of 16, scale > 0)");
+  const bool chunk = variant == 0 ? nc::paged_chunk_takes(a) : variant == 2;
   const nc::PagedPlan p = chunk ? nc::paged_chunk_plan(a) : nc::paged_rows_plan(a);
   a.splits = p.splits, a.split_keys = p.split_keys;
   Tensor work;
@@ -160,9 +162,9 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
 
 Tensor paged_chunk_attention(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, const Tensor& page_table,
                              const Tensor& seq_lens, const OptTensor& q_lens, int64_t window_left, double scale,
-                             const OptTensor& k_scale, const OptTensor& v_scale) {
+                             const OptTensor& k_scale, const OptTensor& v_scale, int64_t variant) {
   return paged_attention("paged_chunk_attention", q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale,
-                         k_scale, v_scale);
+                         k_scale, v_scale, variant);
 }
 
 Tensor paged_decode_attention_mx(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, const Tensor& k_scale,
@@ -170,7 +172,7 @@ Tensor paged_decode_attention_mx(const Tensor& q, const Tensor& k_pool, const Te
                                  int64_t window_left, double scale) {
   TORCH_CHECK(q.dim() == 3, "paged_decode_attention_mx: q must be [B, H, D]");
   return paged_attention("paged_decode_attention_mx", q.unsqueeze(1), k_pool, v_pool, page_table, seq_lens, OptTensor(),
-                         window_left, scale, k_scale, v_scale).squeeze(1);
+                         window_left, scale, k_scale, v_scale, 0).squeeze(1);
 }
 
 Tensor sample_rows(const Tensor& logits, const Tensor& u, double temperature, int64_t top_k, double top_p, double min_p,

@@ -505,10 +505,13 @@ def paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, s
 
 
 def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, window_left=-1, scale=None,
-                          k_scale=None, v_scale=None):
+                          k_scale=None, v_scale=None, variant=0):
+    """variant 0 (default): the faster kernel for these sizes; 1: `csrc/cuda/paged_rows.cu` (few rows per kv head), any
+    size; 2: `csrc/cuda/paged_chunk.cu` (many rows), pages of a multiple of 16 tokens, scale > 0."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    return _C.paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale)
+    return _C.paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale,
+                                    variant)
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):

@@ -109,6 +109,13 @@ def _run(c, window, decode=False, scale=None):
     return out
 
 
+def _variants(c, window, scale):
+    """The outputs of both kernels, where both take the call."""
+    K = ops.cuda_module()
+    for v in (1, 2) if c["k"].shape[1] % 16 == 0 and (scale is None or scale > 0) else (1,):
+        yield K.paged_chunk_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["q_lens"], window, scale, c["ks"], c["vs"], v)
+
+
 def _hold(c, window, decode=False, scale=None):
     out = _run(c, window, decode, scale)
     assert out.shape == c["q"].shape and out.is_contiguous()
@@ -118,6 +125,9 @@ def _hold(c, window, decode=False, scale=None):
     bad = ~(off <= bound)
     assert not bool(bad.any()), (int(bad.sum()), float((off - bound).max()), bad.nonzero()[0].tolist())
     assert torch.equal(out, _run(c, window, decode, scale))          # the same bits again
+    if not decode:
+        for other in _variants(c, window, scale):
+            assert bool(((other.double() - want).abs() <= bound).all())
     _status()
 
 
@@ -189,7 +199,9 @@ def test_unusable_pages_are_left_out_and_recorded(mx, T):
     with pytest.raises(RuntimeError, match="outside its table"):
         _status()
     want, bound = U.attention(c["q"], U.pool_values(c["k"], c["ks"]), U.pool_values(c["v"], c["vs"]), c["table"], c["lens"], None, -1)
-    assert bool(((out.double() - want).abs() <= bound).all())
+    for o in [out, *_variants(c, -1, None)]:
+        assert bool(((o.double() - want).abs() <= bound).all())
+    ops.cuda_module()._C.reset_status(0)
     c["table"] = c["table"][:, :5].contiguous()         # a table shorter than the sequence
     c["table"][0, 2], c["table"][1, 4] = 0, 0
     c["lens"] = torch.tensor([200, 90], dtype=torch.int32, device="cuda")
@@ -205,6 +217,10 @@ def test_attention_on_another_stream_and_in_graphs(mx):
     """Two captured graphs and eager calls in between, on streams of their own: each has its own workspace."""
     c = [U.paged_case(s, 2, 3, 4, 2, 128, 16, [700, 1500], [3, 2], mx=mx, device="cuda") for s in (1, 2)]
     want = [_run(x, -1) for x in c]
+    many = next(iter(list(_variants(c[0], -1, None))[1:]))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        assert torch.equal(many, list(_variants(c[0], -1, None))[1])
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     graphs, outs = [], []
