@@ -3,10 +3,11 @@
 // Rows are (query token, head of the group): the heads that share a kv head are packed into the 128-row tiles of one CTA
 // (the largest power of two that divides the group), so keys and values are read once for all of them and a chunk
 // of a few tokens still fills a tile. A CTA takes two such tiles and walks the keys that either sees, 128 at a time:
-//   warps 0..3, 4..7  softmax of row tile 0 and 1: a thread owns a row; P replaces S in tensor memory as bf16
-//   warp 8            tcgen05.mma: S^x = Q^x K^T, O^x += P^x V, both in tensor memory all along
-//   warp 9            TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
-//   warps 10..13 (K), 14..17 (V)  on MXFP8 pages: codes are copied (cp.async) one tile ahead, spread to bf16, multiplied by their
+//   warps 0..7, 8..15 softmax of row tile 0 and 1: two threads share a row, 64 keys each (one thread per row left a
+//                     scheduler with one warp to issue from); P replaces S in tensor memory as bf16
+//   warp 16           tcgen05.mma: S^x = Q^x K^T, O^x += P^x V, both in tensor memory all along
+//   warp 17           TMA: Q; on bf16 pages also K and V, one 16-token box per page and 64 channels
+//   warps 18..21 (K), 22..25 (V)  on MXFP8 pages: codes are copied (cp.async) one tile ahead, spread to bf16, multiplied by their
 //                     block's power of two (exact) and stored in the operands' 128-byte swizzled layout
 // The products run in the order O0(j), S0(j + 1), O1(j), S1(j + 1): while one tile's softmax works, the other tile's
 // products do, and S(j + 1) needs no barrier of its own, because it follows the product that read P(j) out of its columns.
@@ -36,6 +37,7 @@ namespace {
 
 constexpr int BQ = 128;    // rows per tile (TMEM lanes)
 constexpr int NQ = 2;      // row tiles per CTA
+constexpr int kSoft = 8;   // softmax warps per row tile
 constexpr int BKV = 128;   // keys per step
 constexpr int KVS = 2;     // stages of K and of V
 constexpr int kBox = 16;   // tokens per TMA box: a page holds a multiple of it
@@ -69,9 +71,11 @@ struct ChunkLayout {
   static constexpr int kRaw = MX ? BKV * D : 0;                // codes of a tile, one side, as they lie in memory
   static constexpr int kOffRaw = kOffV + KVS * kKV;            // K, V
   static constexpr int kOffScale = kOffRaw + 2 * kRaw;         // scale bytes [BKV][D / 32], K, V
-  static constexpr int kOffBar = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);
-  static constexpr int kTotal = kOffBar + 512 + 1024;
-  static constexpr int kThreads = (NQ * 4 + 2 + (MX ? 8 : 0)) * 32;
+  static constexpr int kOffRow = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);   // bf16 [NQ][2][BQ]: between a row's two threads
+  static constexpr int kOffBar = kOffRow + NQ * 2 * BQ * 2;
+  static constexpr int kTotal = kOffBar + 256;
+  static_assert(kTotal <= 227 * 1024, "shared memory of one CTA");
+  static constexpr int kThreads = (NQ * kSoft + 2 + (MX ? 8 : 0)) * 32;
 };
 
 struct ChunkParams {
@@ -87,8 +91,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   using L = ChunkLayout<D, MX>;
   constexpr int DC = D / 64;
   const PagedAttnArgs& a = p.a;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023) != 0) {   // the operands' swizzle wants it; there is no room to align by hand
+    if (threadIdx.x == 0 && a.status != nullptr) atomicCAS(a.status, 0, kErrWaitOther);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t* q_full = bars + 0;
   uint64_t* k_full = bars + 1;
@@ -142,13 +149,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     for (int x = 0; x < NQ; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[x], kSoft);
       mbar_init(&o_final[x], 1);
     }
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == NQ * 4) {
+  if (warp == NQ * kSoft) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -168,7 +175,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   auto tmem_S = [&](int x) { return tmem_base + x * BKV; };
   auto tmem_O = [&](int x) { return tmem_base + 256 + x * 128; };
 
-  if (warp == NQ * 4) {
+  if (warp == NQ * kSoft) {
     // ---------------------------------------------------------------- MMA issuer
     // The whole warp walks the loop and waits, one elected thread issues: control flow and descriptors stay uniform
     // (a single lane that ran it alone took 44 clocks to issue a product).
@@ -247,7 +254,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
       }
     }
-  } else if (warp == NQ * 4 + 1) {
+  } else if (warp == NQ * kSoft + 1) {
     // ---------------------------------------------------------------- TMA: Q, and bf16 keys and values
     if (lane == 0) {
       mbar_expect_tx(q_full, NQ * L::kQ);
@@ -316,14 +323,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const unsigned long long t0 = globaltimer_ns();
       while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-  } else if (MX && warp >= NQ * 4 + 2) {
+  } else if (MX && warp >= NQ * kSoft + 2) {
     // ---------------------------------------------------------------- MXFP8 keys and values -> bf16 operands
     if constexpr (MX) {
       constexpr int U = D / 16;                 // 16-code pieces of a row
       constexpr int N = BKV * U / 128;          // pieces per thread and side: rows t / U + i * (128 / U)
       constexpr int kRows = 128 / U, kBoxStep = kRows / kBox;
-      const int side = (warp - (NQ * 4 + 2)) >> 2;   // 0: keys, 1: values
-      const int t = (threadIdx.x - (NQ * 4 + 2) * 32) & 127;
+      const int side = (warp - (NQ * kSoft + 2)) >> 2;   // 0: keys, 1: values
+      const int t = (threadIdx.x - (NQ * kSoft + 2) * 32) & 127;
       const int row0 = t / U, u = t % U, in_box = row0 % kBox, box0 = row0 / kBox;
       const uint32_t stride = static_cast<uint32_t>(p.KV) * D, s_stride = static_cast<uint32_t>(p.KV) * a.page_size * (D / 32);
       const uint8_t* codes = static_cast<const uint8_t*>(side ? a.v_pool : a.k_pool) + static_cast<long long>(in_box) * stride + kvh * D + u * 16;
@@ -423,8 +430,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    const int x = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
+    const int x = warp / kSoft, half = (warp >> 2) & 1;   // this thread's 64 of the 128 keys of a step
+    const int row = (warp & 3) * 32 + lane;      // (a warp reaches the 32 TMEM lanes of its number modulo 4)
+    const int pair_bar = 1 + x * 4 + (warp & 3);   // named barrier of the two warps that share 32 rows
+    __nv_bfloat16* const row_max = reinterpret_cast<__nv_bfloat16*>(smem + L::kOffRow) + x * 2 * BQ + row;   // [half * BQ]
     const int r = r0 + x * BQ + row;             // row of the pack
     const bool row_in = x * BQ + row < row_count, real = r < rg.n * G;
     const int qpos = real ? rg.base + r / G : -1;
@@ -435,48 +444,47 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const float sl = a.scale * 1.4426950408889634f;
     float m_ref = -1.0e30f, l_run = 0.0f;
     bool ok = true;
-    float sv[64];
-    for (int i = 0; i < n_x && ok; ++i) {
-      const int kv0 = (lo[x] + i) * BKV;
-      const bool need_mask = any_bad || kv0 + BKV - 1 > pos_min || (a.window_left >= 0 && kv0 < pos_max - a.window_left) || kv0 + BKV > rg.hi;
-      // scores of 64 keys, unseen ones -infinity: the maximum wants all 128 first, so the first half is read twice
-      auto load = [&](int half) {
-        uint32_t r0v[32], r1v[32];
-        tmem_ld_32x32(tmem_S(x) + half * 64 + lane_sel, r0v);
-        tmem_ld_32x32(tmem_S(x) + half * 64 + 32 + lane_sel, r1v);
+    float sv[32];
+    for (int i = 0; i < n_x; ++i) {
+      const int kv0 = (lo[x] + i) * BKV + half * 64;
+      const bool need_mask = any_bad || kv0 + 63 > pos_min || (a.window_left >= 0 && kv0 < pos_max - a.window_left) || kv0 + 64 > rg.hi;
+      // scores of 32 keys, unseen ones -infinity: the maximum wants all first, so one of the two pieces is read twice
+      auto load = [&](int piece) {
+        uint32_t rv[32];
+        tmem_ld_32x32(tmem_S(x) + half * 64 + piece * 32 + lane_sel, rv);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) sv[e] = __uint_as_float(r0v[e]), sv[32 + e] = __uint_as_float(r1v[e]);
+        for (int e = 0; e < 32; ++e) sv[e] = __uint_as_float(rv[e]);
         if (!need_mask) return;
-        // keys [k_lo, k_hi) of the half are seen by the row; the rest cannot be told from seen ones by value
-        const int k0 = kv0 + half * 64;
+        // keys [k_lo, k_hi) of the piece are seen by the row; the rest cannot be told from seen ones by value
+        const int k0 = kv0 + piece * 32;
         const int k_hi = min(qpos + 1, rg.hi) - k0, k_lo = (a.window_left >= 0 ? max(0, qpos - a.window_left) : 0) - k0;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) sv[e] = e >= k_lo && e < k_hi ? sv[e] : -CUDART_INF_F;
-        for (int box = 0; any_bad && box < 64 / kBox; ++box) {   // a page outside the pool: its keys are none
+        for (int e = 0; e < 32; ++e) sv[e] = e >= k_lo && e < k_hi ? sv[e] : -CUDART_INF_F;
+        for (int box = 0; any_bad && box < 32 / kBox; ++box) {   // a page outside the pool: its keys are none
           const int key = k0 + box * kBox;
           if (key >= rg.hi || key + kBox <= rg.lo) continue;
           const int page = table[key / a.page_size];
           if (page < 0 || page >= a.num_pages) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e) sv[e] = (e >> 4) == box ? -CUDART_INF_F : sv[e];
+            for (int e = 0; e < 32; ++e) sv[e] = (e >> 4) == box ? -CUDART_INF_F : sv[e];
           }
         }
       };
       auto largest = [&](float m) {
         float mt[4] = {m, m, m, m};   // four chains, three operands an instruction
 #pragma unroll
-        for (int e = 0; e < 64; e += 8)
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
           for (int c = 0; c < 4; ++c) mt[c] = fmaxf(fmaxf(mt[c], sv[e + 2 * c]), sv[e + 2 * c + 1]);
         return fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
       };
-      auto probabilities = [&](int half) {
+      auto probabilities = [&](int piece) {
         const uint64_t sl2 = pack2(sl, sl), m2 = pack2(-m_ref * sl, -m_ref * sl);
-        uint32_t packed[32];
+        uint32_t packed[16];
         uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
-        for (int e = 0; e < 64; e += 2) {
+        for (int e = 0; e < 32; e += 2) {
           float p0, p1;
           unpack2(fma2(pack2(sv[e], sv[e + 1]), sl2, m2), p0, p1);
           p0 = fast_exp2(p0), p1 = fast_exp2(p1);
@@ -486,25 +494,44 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         float l0, l1;
         unpack2(add2(sum[0], sum[1]), l0, l1);
         l_run += l0 + l1;
-        tmem_st_32x32(tmem_S(x) + half * 64 + lane_sel, packed);
+        tmem_st_32x16(tmem_S(x) + half * 64 + piece * 16 + lane_sel, packed);
       };
-      if (!mbar_wait(&s_full[x], i & 1, abort_flag, a.status, kErrWaitTmemFull)) { ok = false; break; }
+      // A wait that gives up leaves the loop's barriers in step: every thread of the tile goes on, on whatever there is.
+      ok = mbar_wait(&s_full[x], i & 1, abort_flag, a.status, kErrWaitTmemFull) && ok;
       tc_fence_after();
-      load(0);
-      float m_tile = largest(-1.0e30f);
       load(1);
+      float m_tile = largest(-1.0e30f);
+      load(0);
       m_tile = largest(m_tile);
+      // Both threads of a row have to use one reference. Whether any of the pair's rows wants a higher one is a barrier
+      // with a vote; only then the maxima themselves are exchanged (rounded up to bf16: all that matters is that both have
+      // the same number, within a step of the largest). The next vote keeps a next exchange behind this one's reads.
       const bool raise = (m_tile - m_ref) * sl > kRescaleThreshold;
-      if (__any_sync(0xffffffffu, raise)) {
+      uint32_t any_raise;
+      asm volatile(
+          "{\n"
+          ".reg .pred p, q;\n"
+          "setp.ne.u32 p, %1, 0;\n"
+          "bar.red.or.pred q, %2, 64, p;\n"
+          "selp.u32 %0, 1, 0, q;\n"
+          "}\n"
+          : "=r"(any_raise)
+          : "r"(static_cast<uint32_t>(raise)), "r"(pair_bar)
+          : "memory");
+      if (any_raise) {
+        const __nv_bfloat16 up = __float2bfloat16_ru(m_tile);
+        row_max[half * BQ] = up;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        m_tile = fmaxf(__bfloat162float(up), __bfloat162float(row_max[(half ^ 1) * BQ]));
         float alpha = 1.0f;
-        if (raise) {
+        if ((m_tile - m_ref) * sl > kRescaleThreshold) {
           alpha = fast_exp2((m_ref - m_tile) * sl);
           m_ref = m_tile;
           l_run *= alpha;
         }
         if (i > 0) {   // the scores of this tile came after the P V product of the one before: O is at rest
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
             uint32_t o[16];
             tmem_ld_32x16(tmem_O(x) + c * 16 + lane_sel, o);
             tmem_ld_wait();
@@ -514,24 +541,31 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
         }
       }
+      probabilities(0);   // into the place of the first 16 of the 32 columns that are in registers
+      load(1);
       probabilities(1);
-      load(0);
-      probabilities(0);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[x]);
     }
     if (ok && n_x > 0) ok = mbar_wait(&o_final[x], 0, abort_flag, a.status, kErrWaitTmemFull);
+    const bool any = n_x > 0;                 // else O was never written
+    if (any) {   // the row's sum: its halves meet where this tile's Q was, which no product reads any more
+      float* const halves = reinterpret_cast<float*>(smem + L::kOffQ + x * L::kQ) + row;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      if (ok) halves[half * BQ] = l_run;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      if (ok) l_run += halves[(half ^ 1) * BQ];
+    }
     if (ok) {
       tc_fence_after();
-      const bool any = n_x > 0;                 // else O was never written
       if (whole) {
         const bool zero = !any || !real || l_run == 0.0f;
         const float inv_l = 1.0f / l_run;
         __nv_bfloat16* op = out_row(x * BQ + (row_in ? row : 0));
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
           uint32_t w[32];
           if (any) {
             tmem_ld_32x32(tmem_O(x) + c * 32 + lane_sel, w);
@@ -554,7 +588,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                                   a.splits + split) * rw + x * BQ + row;
         float* dst = a.part_o + at * D;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
           uint32_t w[32];
           if (any) {
             tmem_ld_32x32(tmem_O(x) + c * 32 + lane_sel, w);
@@ -569,14 +603,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               *reinterpret_cast<uint4*>(dst + c * 32 + g * 4) = make_uint4(w[g * 4], w[g * 4 + 1], w[g * 4 + 2], w[g * 4 + 3]);
           }
         }
-        if (row_in) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref * sl, any ? l_run : 0.0f);
+        if (row_in && half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref * sl, any ? l_run : 0.0f);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == NQ * 4) {
+  if (warp == NQ * kSoft) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
