@@ -3,10 +3,11 @@
 // A block is 32 channels of one token and head: code = e4m3(x * 2^(127 - b)), value = code * 2^(b - 127) with b from the
 // block's largest magnitude (mx_cache.cuh). Scales being powers of two, scaling is exact in both directions and the code
 // is the only rounding. Both kernels only move bytes (append: 2 read, 1 + 1/32 written per element; read: the reverse),
-// so what counts is that a thread has all its loads in flight at once and that every access is 16 bytes wide: a
-// thread owns 16 channels of one row, two threads share a block and exchange their maxima by one shuffle.
-// The scale pool is laid out [page, head, token, block]: the scales of one page and head, which the attention
-// kernels read together, are contiguous.
+// but at a few hundred bytes a row they run out of instructions before bandwidth if every thread works out its own place:
+// a warp takes a token (several, where they are narrow), finds the place once, and its lanes go over the key AND value
+// row in pieces of 8 channels, neighbouring lanes on neighbouring pieces. Four lanes share a block and exchange their
+// maxima by two shuffles. The scale pool is laid out [page, head, token, block]: the scales of one page and head, which
+// the attention kernels read together, are contiguous.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -24,132 +25,169 @@ namespace nc {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 4;   // pieces of a row that a lane has in flight
 
-// Where the row of (token, head) lives; false: not a usable place (a negative position is simply not one).
-__device__ __forceinline__ bool place(const MxCache& c, int b, int pos, int h, int* status, bool report, long long& row,
-                                      long long& srow) {
-  if (pos < 0) return false;
-  const int lp = pos / c.page_size, slot = pos - lp * c.page_size;
-  const int page = lp < c.max_pages ? c.page_table[static_cast<long long>(b) * c.max_pages + lp] : -1;
-  if (page < 0 || page >= c.num_pages) {
-    if (report && status != nullptr) atomicCAS(status, 0, kErrBadIndex);
-    return false;
-  }
-  row = ((static_cast<long long>(page) * c.page_size + slot) * c.KV + h) * c.D;
-  srow = ((static_cast<long long>(page) * c.KV + h) * c.page_size + slot) * (c.D / 32);
-  return true;
-}
-
-// Index space: [token][K or V][head][D / 16], one thread each.
-struct Unit {
-  int tok, b, h, d0;
-  bool is_v, first;
+// The lanes of a warp: `per` of them to a token, 8 channels each at a time, and so many tokens per warp.
+struct Split {
+  int units, per, tokens;
 };
-__device__ __forceinline__ Unit unit_of(unsigned idx, const MxCache& c, int T) {
-  const unsigned per_head = c.D / 16, per_side = c.KV * per_head;
-  const unsigned side = idx / per_side, rest = idx - side * per_side;
-  Unit u;
-  u.tok = side >> 1, u.is_v = side & 1;
-  u.b = u.tok / T;
-  u.h = rest / per_head;
-  u.d0 = (rest - u.h * per_head) * 16;
-  u.first = rest == 0;
-  return u;
+
+struct Place {
+  long long row, srow;   // of the code pools (the token's row) and scale pools (its first head); row < 0: no usable place
+  int tok, b, t, pos;    // pos < 0: skipped, or not a token of the call
+  int first;             // the lane's first piece
+  bool live;
+};
+__device__ __forceinline__ Place find(const MxCache& c, const int* positions, int B, int T, const Split& s) {
+  Place p;
+  const int lane = threadIdx.x & 31, warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int sub = s.tokens > 1 ? lane / s.per : 0;
+  p.first = lane - sub * s.per;
+  p.tok = warp * s.tokens + sub;
+  p.live = sub < s.tokens && p.tok < B * T;
+  p.pos = p.live ? positions[p.tok] : -1;
+  p.b = T == 1 ? p.tok : p.tok / T;
+  p.t = p.tok - p.b * T;
+  return p;
+}
+__device__ __forceinline__ void look_up(const MxCache& c, int* status, Place& p) {
+  p.row = p.srow = -1;
+  if (p.pos < 0) return;
+  const int lp = p.pos / c.page_size, slot = p.pos - lp * c.page_size;
+  const int page = lp < c.max_pages ? c.page_table[static_cast<long long>(p.b) * c.max_pages + lp] : -1;
+  if (page < 0 || page >= c.num_pages) {
+    if (p.first == 0 && status != nullptr) atomicCAS(status, 0, kErrBadIndex);
+    return;
+  }
+  p.row = (static_cast<long long>(page) * c.page_size + slot) * c.KV * c.D;
+  p.srow = (static_cast<long long>(page) * c.KV * c.page_size + slot) * (c.D / 32);
 }
 
-__global__ void __launch_bounds__(kThreads) kv_append_mx_kernel(const MxCache c, const int* __restrict__ positions, int T,
-                                                                unsigned total, const KvRows kr, const KvRows vr,
-                                                                int* status) {
-  NC_PDL_PROLOGUE();
-  const unsigned idx = blockIdx.x * kThreads + threadIdx.x;
-  const bool live = idx < total;     // the shuffle below wants the whole warp
-  const Unit u = unit_of(live ? idx : 0, c, T);
-  const int pos = live ? positions[u.tok] : -1;
-  uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (pos >= 0) {
-    const KvRows& r = u.is_v ? vr : kr;
-    const uint4* src = reinterpret_cast<const uint4*>(r.ptr + u.b * r.stride_b + (u.tok - u.b * T) * r.stride_t +
-                                                      u.h * r.stride_h + u.d0);
-    x[0] = src[0], x[1] = src[1];
-  }
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+// Eight values of a block of four neighbouring lanes -> eight codes and the block's scale byte.
+__device__ __forceinline__ uint2 encode(const uint4& x, uint32_t& b) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t mx = 0;   // the larger magnitudes of even and odd channels, as 16-bit fields (magnitude bits order as numbers)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
+  for (int i = 0; i < 4; ++i) mx = __vmaxu2(mx, w[i] & 0x7fff7fffu);
   mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-  const uint32_t amax = max(mx & 0xffffu, mx >> 16);
-  if (pos < 0) return;
-  long long row, srow;
-  if (!place(c, u.b, pos, u.h, status, u.first && !u.is_v, row, srow)) return;
-  const uint32_t b = mx_scale_byte(amax);
-  uint4 code = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);   // a block of NaN
-  if (b != 255u) {
-    const float inv = mx_inverse_scale(b);
-    float f[16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[2 * i] = bf16_lo(w[i]) * inv, f[2 * i + 1] = bf16_hi(w[i]) * inv;
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = mx_to_e4m3x2(f[4 * i], f[4 * i + 1]) | (mx_to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16);
-    code = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-  *reinterpret_cast<uint4*>((u.is_v ? c.v : c.k) + row + u.d0) = code;
-  if ((u.d0 & 16) == 0) (u.is_v ? c.v_scale : c.k_scale)[srow + u.d0 / 32] = static_cast<uint8_t>(b);
+  mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  b = mx_scale_byte(max(mx & 0xffffu, mx >> 16));
+  if (b == 255u) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);   // a block of NaN
+  const float inv = mx_inverse_scale(b);
+  const float f[8] = {bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1]), bf16_lo(w[2]), bf16_hi(w[2]), bf16_lo(w[3]), bf16_hi(w[3])};
+  return mx_pack8(f, inv);
 }
 
-__global__ void __launch_bounds__(kThreads) kv_read_mx_kernel(const MxCache c, const int* __restrict__ positions, int T,
-                                                              unsigned total, __nv_bfloat16* __restrict__ k_out,
-                                                              __nv_bfloat16* __restrict__ v_out, int* status) {
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_append_mx_kernel(const MxCache c, const int* __restrict__ positions, int B, int T,
+                                                                const Split s, const KvRows kr, const KvRows vr, int* status) {
   NC_PDL_PROLOGUE();
-  const unsigned idx = blockIdx.x * kThreads + threadIdx.x;
-  if (idx >= total) return;
-  const Unit u = unit_of(idx, c, T);
-  uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  long long row, srow;
-  if (place(c, u.b, positions[u.tok], u.h, status, u.first && !u.is_v, row, srow)) {
-    const uint4 code = *reinterpret_cast<const uint4*>((u.is_v ? c.v : c.k) + row + u.d0);
-    const uint32_t b = (u.is_v ? c.v_scale : c.k_scale)[srow + u.d0 / 32];
-    const uint32_t f1 = mx_factor_first(b) * 0x10001u, f2 = mx_factor_second(b) * 0x10001u;
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&code);
-    uint32_t* r = reinterpret_cast<uint32_t*>(o);
+  Place p = find(c, positions, B, T, s);
+  const __nv_bfloat16* ks = kr.ptr + p.b * kr.stride_b + p.t * kr.stride_t;
+  const __nv_bfloat16* vs = vr.ptr + p.b * vr.stride_b + p.t * vr.stride_t;
+  bool looked = false;
+  // every lane of the warp goes round as often: the shuffles want all of them
+  for (int u0 = 0; u0 < s.units; u0 += kBatch * s.per) {
+    uint4 xk[kBatch], xv[kBatch];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      mx_spread(w[i], r[2 * i], r[2 * i + 1]);
-      r[2 * i] = mul_bf16x2(mul_bf16x2(r[2 * i], f1), f2);
-      r[2 * i + 1] = mul_bf16x2(mul_bf16x2(r[2 * i + 1], f1), f2);
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = u0 + i * s.per + p.first, h = u / (D / 8), d0 = u % (D / 8) * 8;
+      xk[i] = xv[i] = make_uint4(0, 0, 0, 0);
+      if (u < s.units && p.pos >= 0) {
+        xk[i] = __ldcs(reinterpret_cast<const uint4*>(ks + h * kr.stride_h + d0));
+        xv[i] = __ldcs(reinterpret_cast<const uint4*>(vs + h * vr.stride_h + d0));
+      }
+    }
+    if (!looked) look_up(c, status, p), looked = true;   // (the first rows are on their way meanwhile)
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = u0 + i * s.per + p.first, h = u / (D / 8), d0 = u % (D / 8) * 8;
+      if (u0 + i * s.per >= s.units) break;              // the same for every lane
+      uint32_t bk, bv;
+      const uint2 ck = encode(xk[i], bk), cv = encode(xv[i], bv);
+      if (u < s.units && p.row >= 0) {
+        *reinterpret_cast<uint2*>(c.k + p.row + u * 8) = ck;
+        *reinterpret_cast<uint2*>(c.v + p.row + u * 8) = cv;
+        if ((d0 & 31) == 0) {
+          const long long at = p.srow + static_cast<long long>(h) * c.page_size * (D / 32) + d0 / 32;
+          c.k_scale[at] = static_cast<uint8_t>(bk), c.v_scale[at] = static_cast<uint8_t>(bv);
+        }
+      }
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>((u.is_v ? v_out : k_out) + (static_cast<long long>(u.tok) * c.KV + u.h) * c.D + u.d0);
-  dst[0] = o[0], dst[1] = o[1];
 }
 
-const char* grid_of(const MxCache& c, int B, int T, unsigned& total, unsigned& blocks) {
-  const long long n = 2LL * B * T * c.KV * (c.D / 16);
-  if (n >= (1LL << 32) - kThreads) return "kv_mx: more than 2^32 units of 16 channels in one call";
-  total = static_cast<unsigned>(n);
-  blocks = (total + kThreads - 1) / kThreads;
-  return nullptr;
+__device__ __forceinline__ uint4 decode(const uint2& code, uint32_t b) {
+  const uint32_t f1 = mx_factor_first(b) * 0x10001u, f2 = mx_factor_second(b) * 0x10001u;
+  uint32_t r[4];
+  mx_spread(code.x, r[0], r[1]);
+  mx_spread(code.y, r[2], r[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = mul_bf16x2(mul_bf16x2(r[i], f1), f2);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_read_mx_kernel(const MxCache c, const int* __restrict__ positions, int B, int T,
+                                                              const Split s, __nv_bfloat16* __restrict__ k_out,
+                                                              __nv_bfloat16* __restrict__ v_out, int* status) {
+  NC_PDL_PROLOGUE();
+  Place p = find(c, positions, B, T, s);
+  if (!p.live) return;
+  look_up(c, status, p);
+  const long long out = static_cast<long long>(p.tok) * c.KV * D;
+  for (int u0 = p.first; u0 < s.units; u0 += kBatch * s.per) {
+    uint2 ck[kBatch], cv[kBatch];
+    uint32_t bk[kBatch], bv[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = u0 + i * s.per, h = u / (D / 8), d0 = u % (D / 8) * 8;
+      ck[i] = cv[i] = make_uint2(0, 0), bk[i] = bv[i] = 127;
+      if (u < s.units && p.row >= 0) {
+        ck[i] = *reinterpret_cast<const uint2*>(c.k + p.row + u * 8), cv[i] = *reinterpret_cast<const uint2*>(c.v + p.row + u * 8);
+        const long long at = p.srow + static_cast<long long>(h) * c.page_size * (D / 32) + d0 / 32;
+        bk[i] = c.k_scale[at], bv[i] = c.v_scale[at];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = u0 + i * s.per;
+      if (u >= s.units) break;
+      __stcs(reinterpret_cast<uint4*>(k_out + out + u * 8), decode(ck[i], bk[i]));
+      __stcs(reinterpret_cast<uint4*>(v_out + out + u * 8), decode(cv[i], bv[i]));
+    }
+  }
+}
+
+Split split_of(const MxCache& c) {
+  Split s;
+  s.units = c.KV * (c.D / 8);
+  s.per = s.units < 32 ? s.units : 32;   // a multiple of 8: blocks of four lanes stay together
+  s.tokens = 32 / s.per;
+  return s;
+}
+unsigned blocks_of(const Split& s, int B, int T) {
+  const long long per_cta = static_cast<long long>(s.tokens) * (kThreads / 32);
+  return static_cast<unsigned>((static_cast<long long>(B) * T + per_cta - 1) / per_cta);
 }
 
 }  // namespace
 
 const char* kv_append_mx(const MxCache& c, const int* positions, int B, int T, const KvRows& k, const KvRows& v,
                          int* status, cudaStream_t s) {
-  unsigned total, blocks;
-  if (const char* e = grid_of(c, B, T, total, blocks)) return e;
-  if (total == 0) return nullptr;
-  const cudaError_t e = launch_maybe_pdl(kv_append_mx_kernel, dim3(blocks), dim3(kThreads), 0, s, c, positions, T, total, k,
-                                         v, status);
+  if (B == 0 || T == 0) return nullptr;
+  const Split h = split_of(c);
+  const cudaError_t e = launch_maybe_pdl(c.D == 128 ? kv_append_mx_kernel<128> : kv_append_mx_kernel<64>,
+                                         dim3(blocks_of(h, B, T)), dim3(kThreads), 0, s, c, positions, B, T, h, k, v, status);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
 const char* kv_read_mx(const MxCache& c, const int* positions, int B, int T, __nv_bfloat16* k_out, __nv_bfloat16* v_out,
                        int* status, cudaStream_t s) {
-  unsigned total, blocks;
-  if (const char* e = grid_of(c, B, T, total, blocks)) return e;
-  if (total == 0) return nullptr;
-  const cudaError_t e = launch_maybe_pdl(kv_read_mx_kernel, dim3(blocks), dim3(kThreads), 0, s, c, positions, T, total, k_out,
-                                         v_out, status);
+  if (B == 0 || T == 0) return nullptr;
+  const Split h = split_of(c);
+  const cudaError_t e = launch_maybe_pdl(c.D == 128 ? kv_read_mx_kernel<128> : kv_read_mx_kernel<64>, dim3(blocks_of(h, B, T)),
+                                         dim3(kThreads), 0, s, c, positions, B, T, h, k_out, v_out, status);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
