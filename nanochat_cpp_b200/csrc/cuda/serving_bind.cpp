@@ -65,9 +65,11 @@ nc::MxCache mx_cache(const char* op, const Tensor& k, const Tensor& v, const Ten
 }
 
 // [B, T, heads, D] rows that allow 16-byte loads; a view that does not is copied.
-Tensor row_view(const char* op, const char* name, const Tensor& t) {
-  TORCH_CHECK(t.dim() == 4 && t.scalar_type() == torch::kBFloat16, op, ": ", name, " must be bf16 [B, T, heads, D]");
-  const bool ok = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && aligned16(t);
+Tensor row_view(const char* op, const char* name, const Tensor& t, int dim = 4) {
+  TORCH_CHECK(t.dim() == dim && t.scalar_type() == torch::kBFloat16, op, ": ", name, " must be bf16 ",
+              dim == 4 ? "[B, T, heads, D]" : "[B, heads, D]");
+  bool ok = t.stride(dim - 1) == 1 && aligned16(t);
+  for (int i = 0; i < dim - 1; ++i) ok = ok && t.stride(i) % 8 == 0;
   return ok ? t : t.contiguous();
 }
 
@@ -101,7 +103,7 @@ std::vector<Tensor> kv_read_mx(const Tensor& k_pool, const Tensor& v_pool, const
   const nc::MxCache c = mx_cache("kv_read_mx", k_pool, v_pool, k_scale, v_scale, page_table, positions);
   const int B = positions.size(0), T = positions.size(1);
   const auto opt = k_pool.options().dtype(torch::kBFloat16);
-  Tensor k = torch::empty({B, T, c.KV, c.D}, opt), v = torch::empty({B, T, c.KV, c.D}, opt);
+  Tensor k = at::empty({B, T, c.KV, c.D}, opt), v = at::empty({B, T, c.KV, c.D}, opt);
   const char* err = nc::kv_read_mx(c, positions.data_ptr<int>(), B, T, reinterpret_cast<__nv_bfloat16*>(k.data_ptr()),
                                    reinterpret_cast<__nv_bfloat16*>(v.data_ptr()),
                                    ncbind::device_status(k_pool.get_device()), at::cuda::getCurrentCUDAStream());
@@ -109,17 +111,20 @@ std::vector<Tensor> kv_read_mx(const Tensor& k_pool, const Tensor& v_pool, const
   return {k, v};
 }
 
-// q [B, T, H, D] (any strides that are multiples of 8); the result is dense and of q's shape.
+// q [B, T, H, D], or [B, H, D] for one token each (any strides that are multiples of 8); the result is dense and of q's
+// shape.
 Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool, const Tensor& v_pool, const Tensor& page_table,
                        const Tensor& seq_lens, const OptTensor& q_lens, int64_t window_left, double scale,
                        const OptTensor& k_scale, const OptTensor& v_scale, int64_t variant) {
   const c10::cuda::CUDAGuard g(k_pool.device());
   check_pools(op, k_pool, v_pool, k_scale, v_scale);
   same_device(q_in, k_pool, op, "q");
-  const Tensor q = row_view(op, "q", q_in);
+  const bool one = q_in.dim() == 3;
+  const Tensor q = row_view(op, "q", q_in, one ? 3 : 4);
   nc::PagedAttnArgs a;
-  TORCH_CHECK(q.size(0) <= 65535 && q.size(1) < (1 << 24) && q.size(2) < (1 << 16), op, ": q is too large");
-  a.B = q.size(0), a.T = q.size(1), a.H = q.size(2), a.D = q.size(3), a.KV = k_pool.size(2);
+  const int h = one ? 1 : 2;   // dimension of the heads
+  TORCH_CHECK(q.size(0) <= 65535 && (one || q.size(1) < (1 << 24)) && q.size(h) < (1 << 16), op, ": q is too large");
+  a.B = q.size(0), a.T = one ? 1 : q.size(1), a.H = q.size(h), a.D = q.size(h + 1), a.KV = k_pool.size(2);
   TORCH_CHECK(k_pool.size(3) == a.D && a.H > 0 && a.H % a.KV == 0, op,
               ": heads must be a multiple of kv heads, and q and the pools must have one head_dim");
   check_table(op, page_table, a.B, k_pool);
@@ -130,10 +135,10 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   };
   check_lens(seq_lens, "seq_lens");
   if (q_lens.has_value()) check_lens(*q_lens, "q_lens");
-  Tensor out = torch::empty({a.B, a.T, a.H, a.D}, q.options());
+  Tensor out = at::empty(q.sizes(), q.options());
   if (out.numel() == 0) return out;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
-  a.q_stride_b = q.stride(0), a.q_stride_t = q.stride(1), a.q_stride_h = q.stride(2);
+  a.q_stride_b = q.stride(0), a.q_stride_t = one ? a.H * static_cast<long long>(a.D) : q.stride(1), a.q_stride_h = q.stride(h);
   a.k_pool = k_pool.data_ptr(), a.v_pool = v_pool.data_ptr();
   if (k_scale.has_value()) a.k_scale = k_scale->data_ptr<uint8_t>(), a.v_scale = v_scale->data_ptr<uint8_t>();
   a.page_table = page_table.data_ptr<int>();
@@ -151,7 +156,7 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   a.splits = p.splits, a.split_keys = p.split_keys;
   Tensor work;
   if (p.splits > 1) {   // a buffer of its own per call: calls on other streams or in other graphs never share it
-    work = torch::empty({p.part_o + p.part_ml}, q.options().dtype(torch::kFloat32));
+    work = at::empty({p.part_o + p.part_ml}, q.options().dtype(torch::kFloat32));
     a.part_o = work.data_ptr<float>(), a.part_ml = a.part_o + p.part_o;
   }
   const auto stream = at::cuda::getCurrentCUDAStream();
@@ -163,6 +168,7 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
 Tensor paged_chunk_attention(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, const Tensor& page_table,
                              const Tensor& seq_lens, const OptTensor& q_lens, int64_t window_left, double scale,
                              const OptTensor& k_scale, const OptTensor& v_scale, int64_t variant) {
+  TORCH_CHECK(q.dim() == 4, "paged_chunk_attention: q must be [B, T, H, D]");
   return paged_attention("paged_chunk_attention", q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale,
                          k_scale, v_scale, variant);
 }
@@ -171,8 +177,8 @@ Tensor paged_decode_attention_mx(const Tensor& q, const Tensor& k_pool, const Te
                                  const Tensor& v_scale, const Tensor& page_table, const Tensor& seq_lens,
                                  int64_t window_left, double scale) {
   TORCH_CHECK(q.dim() == 3, "paged_decode_attention_mx: q must be [B, H, D]");
-  return paged_attention("paged_decode_attention_mx", q.unsqueeze(1), k_pool, v_pool, page_table, seq_lens, OptTensor(),
-                         window_left, scale, k_scale, v_scale, 0).squeeze(1);
+  return paged_attention("paged_decode_attention_mx", q, k_pool, v_pool, page_table, seq_lens, OptTensor(), window_left,
+                         scale, k_scale, v_scale, 0);
 }
 
 Tensor sample_rows(const Tensor& logits, const Tensor& u, double temperature, int64_t top_k, double top_p, double min_p,
@@ -202,7 +208,7 @@ Tensor sample_rows(const Tensor& logits, const Tensor& u, double temperature, in
   if (top_p_rows.has_value()) rows(*top_p_rows, torch::kFloat32, "top_p"), a.top_p_rows = top_p_rows->data_ptr<float>();
   if (min_p_rows.has_value()) rows(*min_p_rows, torch::kFloat32, "min_p"), a.min_p_rows = min_p_rows->data_ptr<float>();
   if (top_k_rows.has_value()) rows(*top_k_rows, torch::kInt32, "top_k"), a.top_k_rows = top_k_rows->data_ptr<int>();
-  Tensor out = torch::empty({R}, logits.options().dtype(torch::kInt64));
+  Tensor out = at::empty({R}, logits.options().dtype(torch::kInt64));
   a.out = reinterpret_cast<long long*>(out.data_ptr<int64_t>());
   const char* err = nc::sample_rows(a, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(err == nullptr, err);

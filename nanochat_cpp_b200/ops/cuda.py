@@ -489,19 +489,24 @@ def paged_decode_attention(q, k_pool, v_pool, page_table, seq_lens, window_left=
 # ---------------------------------------------------------------------------
 # MXFP8 KV cache, attention of new tokens over the pages, sampling
 # ---------------------------------------------------------------------------
+# looked up once: for calls of a few microseconds the proxy's attribute look-up counts
+_kv_append_mx, _kv_read_mx, _sample_rows = _C.kv_append_mx, _C.kv_read_mx, _C.sample_rows
+_paged_decode_attention_mx, _paged_chunk_attention = _C.paged_decode_attention_mx, _C.paged_chunk_attention
+
+
 def kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new):
-    _C.kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new)
+    _kv_append_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions, k_new, v_new)
 
 
 def kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions):
-    k, v = _C.kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions)
+    k, v = _kv_read_mx(k_pool, v_pool, k_scale, v_scale, page_table, positions)
     return k, v
 
 
 def paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left=-1, scale=None):
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    return _C.paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left, scale)
+    return _paged_decode_attention_mx(q, k_pool, v_pool, k_scale, v_scale, page_table, seq_lens, window_left, scale)
 
 
 def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, window_left=-1, scale=None,
@@ -510,17 +515,17 @@ def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, 
     size; 2: `csrc/cuda/paged_chunk.cu` (many rows), pages of a multiple of 16 tokens, scale > 0."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    return _C.paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale,
+    return _paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens, window_left, scale, k_scale, v_scale,
                                     variant)
 
 
 def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     rows = [x if isinstance(x, torch.Tensor) else None for x in (temperature, top_k, top_p, min_p)]
-    if rows == [None, None, None, None]:
-        return _C.sample_rows(logits, u, temperature, top_k, top_p, min_p, None, None, None, None)
+    if all(r is None for r in rows):
+        return _sample_rows(logits, u, temperature, top_k, top_p, min_p, None, None, None, None)
     t, k, tp, mp = (d if r is not None else x for x, r, d in
                     zip((temperature, top_k, top_p, min_p), rows, (1.0, 0, 1.0, 0.0)))
-    return _C.sample_rows(logits, u, t, k, tp, mp, *rows)
+    return _sample_rows(logits, u, t, k, tp, mp, *rows)
 
 
 def __getattr__(name):
