@@ -21,10 +21,6 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
 // four significant bits, and every product of the ordinary range is a normal bf16 number. The multiplier
 // 2^(b - 127 + 120) has a bf16 exponent field for b <= 134 (blocks up to 57344); above that a second factor takes the rest.
 // The codes 0x7f / 0xff (NaN) only occur in blocks of scale 255, whose factor is NaN.
-struct MxFactor {
-  uint32_t first;   // bf16 bits
-  uint32_t second;  // bf16 bits of the rest, 1.0 unless b > 134
-};
 __device__ __forceinline__ uint32_t mx_factor_first(uint32_t b) { return (b < 134u ? b + 120u : 254u) << 7; }
 __device__ __forceinline__ uint32_t mx_factor_second(uint32_t b) {
   return b <= 134u ? 0x3f80u : (b == 255u ? 0x7fc0u : (b - 134u + 127u) << 7);

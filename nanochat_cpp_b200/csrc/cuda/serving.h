@@ -38,7 +38,7 @@ struct PagedAttnArgs {
   const int* page_table = nullptr;                              // [B, max_pages]
   int max_pages = 0, page_size = 16, num_pages = 0;
   const int* seq_lens = nullptr;                                // [B], new tokens included
-  const int* q_lens = nullptr;                                  // [B]; null: min(T, seq_lens) for T = 1, else T
+  const int* q_lens = nullptr;                                  // [B]; null: T for every sequence
   int window_left = -1;
   float scale = 1.0f;
   __nv_bfloat16* out = nullptr;                                 // dense [B, T, H, D]
