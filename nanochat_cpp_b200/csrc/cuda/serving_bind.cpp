@@ -64,13 +64,14 @@ nc::MxCache mx_cache(const char* op, const Tensor& k, const Tensor& v, const Ten
   return c;
 }
 
-// [B, T, heads, D] rows that allow 16-byte loads; a view that does not is copied.
+// [B, T, heads, D] rows that allow 16-byte loads and tensor maps; a view that does not is copied (by clone: contiguous()
+// returns a dense view as it is, whatever its address).
 Tensor row_view(const char* op, const char* name, const Tensor& t, int dim = 4) {
   TORCH_CHECK(t.dim() == dim && t.scalar_type() == torch::kBFloat16, op, ": ", name, " must be bf16 ",
               dim == 4 ? "[B, T, heads, D]" : "[B, heads, D]");
   bool ok = t.stride(dim - 1) == 1 && aligned16(t);
-  for (int i = 0; i < dim - 1; ++i) ok = ok && t.stride(i) % 8 == 0;
-  return ok ? t : t.contiguous();
+  for (int i = 0; i < dim - 1; ++i) ok = ok && t.stride(i) > 0 && t.stride(i) % 8 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 nc::KvRows kv_rows(const Tensor& t) {

@@ -245,6 +245,45 @@ def test_attention_on_another_stream_and_in_graphs(mx):
     _status()
 
 
+def _views(t):
+    """The numbers of t in dense rows at an odd address, broadcast along the first dimension, and with an odd stride of a
+    dimension of one."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+    odd = flat[1:].view(t.shape)
+    odd.copy_(t)
+    yield odd
+    yield t[:1].expand(t.shape)
+    one = t[:1].contiguous()
+    yield torch.as_strided(one, one.shape, (5, *one.stride()[1:]))
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_rows_at_any_address(mx):
+    c = U.paged_case(6, 2, 40, 4, 2, 128, 16, [90, 300], [40, 33], mx=mx, device="cuda")
+    for q in _views(c["q"]):
+        B = q.shape[0]
+        part = dict(c, q=q, table=c["table"][:B].contiguous(), lens=c["lens"][:B], q_lens=c["q_lens"][:B])
+        for a, b in zip(_variants(part, -1, None), _variants(dict(part, q=q.clone(memory_format=torch.contiguous_format)), -1, None)):
+            assert torch.equal(a, b)
+    _status()
+
+
+def test_append_of_rows_at_any_address():
+    k = _rows(3, 2, 5, 2, 128).cuda()
+    table = torch.arange(2, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    for view in _views(k):
+        B = view.shape[0]
+        pos = torch.arange(5, dtype=torch.int32, device="cuda").repeat(B, 1)
+        got = []
+        for x in (view, view.clone(memory_format=torch.contiguous_format)):
+            pools = [torch.zeros(2, 16, 2, 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+            pools += [torch.zeros(2, 2, 16, 4, dtype=torch.uint8, device="cuda") for _ in range(2)]
+            ops.kv_append_mx(*pools, table[:B].contiguous(), pos, x, x)
+            got.append(pools)
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    _status()
+
+
 # ------------------------------------------------------------------------------------------------ sampling
 def _logits(seed, R, V, bf16, scale=2.5):
     g = torch.Generator().manual_seed(seed)
