@@ -574,6 +574,11 @@ cudaError_t launch_shape(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace
 
+bool paged_rows_can(const PagedAttnArgs& a) {
+  const int G = a.H / a.KV, rows = 8 * row_tiles(a);
+  return static_cast<long long>(a.KV) * ((static_cast<long long>(a.T) * G + rows - 1) / rows) <= 65535;
+}
+
 PagedPlan paged_rows_plan(const PagedAttnArgs& a) {
   const int G = a.H / a.KV, rows = 8 * row_tiles(a), blocks = (a.T * G + rows - 1) / rows;
   long long keys = static_cast<long long>(a.max_pages) * a.page_size;

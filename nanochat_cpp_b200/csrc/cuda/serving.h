@@ -55,6 +55,8 @@ struct PagedPlan {
 };
 PagedPlan paged_rows_plan(const PagedAttnArgs& a);
 const char* paged_rows_attention(const PagedAttnArgs& a, cudaStream_t s);
+// Whether the rows make a grid that can be launched.
+bool paged_rows_can(const PagedAttnArgs& a);
 // The same for many rows per kv head: whether it can take these arguments, and whether it is the faster one for them.
 bool paged_chunk_can(const PagedAttnArgs& a);
 bool paged_chunk_takes(const PagedAttnArgs& a);

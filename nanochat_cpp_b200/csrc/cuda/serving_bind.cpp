@@ -121,11 +121,14 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   check_pools(op, k_pool, v_pool, k_scale, v_scale);
   same_device(q_in, k_pool, op, "q");
   const bool one = q_in.dim() == 3;
-  const Tensor q = row_view(op, "q", q_in, one ? 3 : 4);
   nc::PagedAttnArgs a;
   const int h = one ? 1 : 2;   // dimension of the heads
-  TORCH_CHECK(q.size(0) <= 65535 && (one || q.size(1) < (1 << 24)) && q.size(h) < (1 << 16), op, ": q is too large");
-  a.B = q.size(0), a.T = one ? 1 : q.size(1), a.H = q.size(h), a.D = q.size(h + 1), a.KV = k_pool.size(2);
+  // row numbers are ints in the kernels: T * H with room for the last tile
+  TORCH_CHECK(q_in.dim() == h + 2 && q_in.size(0) <= 65535 && q_in.size(h) < (1 << 16) &&
+                  (one || (q_in.size(1) < (1 << 24) && q_in.size(1) * q_in.size(h) < (1LL << 30))) &&
+                  q_in.numel() / std::max<int64_t>(q_in.size(h + 1), 1) < (1LL << 32),
+              op, ": q is too large");
+  a.B = q_in.size(0), a.T = one ? 1 : q_in.size(1), a.H = q_in.size(h), a.D = q_in.size(h + 1), a.KV = k_pool.size(2);
   TORCH_CHECK(k_pool.size(3) == a.D && a.H > 0 && a.H % a.KV == 0, op,
               ": heads must be a multiple of kv heads, and q and the pools must have one head_dim");
   check_table(op, page_table, a.B, k_pool);
@@ -136,6 +139,16 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   };
   check_lens(seq_lens, "seq_lens");
   if (q_lens.has_value()) check_lens(*q_lens, "q_lens");
+  a.page_size = k_pool.size(1), a.num_pages = k_pool.size(0), a.scale = static_cast<float>(scale);
+  a.max_pages = page_table.size(1);
+  a.window_left = window_left < 0 ? -1 : static_cast<int>(std::min<int64_t>(window_left, 1 << 30));
+  const bool can = nc::paged_chunk_can(a);
+  TORCH_CHECK(variant >= 0 && variant <= 2 && (variant != 2 || can), op,
+              ": variant must be 0 (by size), 1 (few rows) or 2 (many rows: page_size a multiple of 16, scale > 0)");
+  const bool rows_can = nc::paged_rows_can(a);
+  const bool chunk = variant == 0 ? nc::paged_chunk_takes(a) || (can && !rows_can) : variant == 2;
+  TORCH_CHECK(chunk || rows_can, op, ": so many new tokens need pages of a multiple of 16 tokens and a scale above 0");
+  const Tensor q = row_view(op, "q", q_in, one ? 3 : 4);
   Tensor out = at::empty(q.sizes(), q.options());
   if (out.numel() == 0) return out;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
@@ -143,16 +156,10 @@ Tensor paged_attention(const char* op, const Tensor& q_in, const Tensor& k_pool,
   a.k_pool = k_pool.data_ptr(), a.v_pool = v_pool.data_ptr();
   if (k_scale.has_value()) a.k_scale = k_scale->data_ptr<uint8_t>(), a.v_scale = v_scale->data_ptr<uint8_t>();
   a.page_table = page_table.data_ptr<int>();
-  a.max_pages = page_table.size(1), a.page_size = k_pool.size(1), a.num_pages = k_pool.size(0);
   a.seq_lens = seq_lens.data_ptr<int>();
   if (q_lens.has_value()) a.q_lens = q_lens->data_ptr<int>();
-  a.window_left = window_left < 0 ? -1 : static_cast<int>(std::min<int64_t>(window_left, 1 << 30));
-  a.scale = static_cast<float>(scale);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.status = ncbind::device_status(k_pool.get_device());
-  TORCH_CHECK(variant >= 0 && variant <= 2 && (variant != 2 || nc::paged_chunk_can(a)), op,
-              ": variant must be 0 (by size), 1 (few rows) or 2 (many rows: page_size a multiple of 16, scale > 0)");
-  const bool chunk = variant == 0 ? nc::paged_chunk_takes(a) : variant == 2;
   const nc::PagedPlan p = chunk ? nc::paged_chunk_plan(a) : nc::paged_rows_plan(a);
   a.splits = p.splits, a.split_keys = p.split_keys;
   Tensor work;

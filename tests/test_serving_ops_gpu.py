@@ -245,6 +245,43 @@ def test_attention_on_another_stream_and_in_graphs(mx):
     _status()
 
 
+@pytest.mark.parametrize("T,H,page,scale,why", [(1 << 22, 1, 8, None, "so many new tokens"), (1 << 22, 1, 16, -1.0, "so many new tokens"),
+                                                (1 << 22, 1, 16, 0.0, "so many new tokens"), (1 << 24, 1, 16, None, "too large"),
+                                                (1 << 20, 1024, 16, None, "too large")])
+def test_chunks_too_long_are_refused(T, H, page, scale, why):
+    """Nothing is allocated for them: q is broadcast."""
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda").expand(1, T, H, 64)
+    k = torch.zeros(2, page, 1, 64, dtype=torch.bfloat16, device="cuda")
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match=why):
+        ops.paged_chunk_attention(q, k, k.clone(), table, lens, lens, -1, scale)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+@pytest.mark.parametrize("T", [1, 90])
+def test_scales_that_are_not_positive(mx, scale, T):
+    _hold(U.paged_case(21, 2, T, 4, 2, 64, 16, [T + 600, T + 3], [T, max(1, T - 2)], mx=mx, device="cuda"), -1, scale=scale)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_two_calls_at_once(mx):
+    """Calls on two streams, in flight together, of both kernels: the results are those of calls one after the other."""
+    c = [U.paged_case(s, 4, 64, 4, 2, 128, 16, [2000, 700, 64, 1500], [64, 3, 64, 50], mx=mx, device="cuda") for s in (1, 2)]
+    want = [list(_variants(x, -1, None)) for x in c]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(list(_variants(c[i], -1, None)))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+    _status()
+
+
 def _views(t):
     """The numbers of t in dense rows at an odd address, broadcast along the first dimension, and with an odd stride of a
     dimension of one."""
