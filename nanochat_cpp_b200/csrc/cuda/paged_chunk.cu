@@ -18,8 +18,8 @@
 // (a place behind the sequence's end) may be NaN, and 0 * NaN is not 0.
 // The running maximum is raised only when a tile exceeds it by more than 2^8: then the thread rescales its O row in tensor
 // memory. Bounds, per 128 x 128 tile: 1024 clocks for the exponentials (16 a clock and SM), 1024 for the two products.
-// Measured (B200, D = 128): 2 x 2048 over 18k keys 386 us on bf16 pages (866 TFLOP/s), 480 on MXFP8 (696); 8 ragged
-// prompts up to 2048, window 1024, 92 us.
+// Measured (B200, D = 128): 2 x 2048 over 18k keys 386 us on bf16 pages (866 TFLOP/s), 482 on MXFP8 (693); 8 ragged
+// prompts up to 2048, window 1024, 93 us.
 // grid: (blocks of 256 rows x key runs, kv heads x head packs, sequences), the blocks that see most first.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -73,8 +73,8 @@ struct ChunkLayout {
   static constexpr int kRaw = MX ? BKV * D : 0;                // codes of a tile, one side, as they lie in memory
   static constexpr int kOffRaw = kOffV + KVS * kKV;            // K, V
   static constexpr int kOffScale = kOffRaw + 2 * kRaw;         // scale bytes [BKV][D / 32], K, V
-  static constexpr int kOffRow = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);   // bf16 [NQ][2][BQ]: between a row's two threads
-  static constexpr int kOffBar = kOffRow + NQ * 2 * BQ * 2;
+  static constexpr int kOffRow = kOffScale + (MX ? 2 * BKV * (D / 32) : 0);   // fp32 [NQ][BQ]: between a row's two threads
+  static constexpr int kOffBar = kOffRow + NQ * BQ * 4;
   static constexpr int kTotal = kOffBar + 256;
   static_assert(kTotal <= 227 * 1024, "shared memory of one CTA");
   static constexpr int kThreads = (NQ * kSoft + 2 + (MX ? 8 : 0)) * 32;
@@ -435,7 +435,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const int x = warp / kSoft, half = (warp >> 2) & 1;   // this thread's 64 of the 128 keys of a step
     const int row = (warp & 3) * 32 + lane;      // (a warp reaches the 32 TMEM lanes of its number modulo 4)
     const int pair_bar = 1 + x * 4 + (warp & 3);   // named barrier of the two warps that share 32 rows
-    __nv_bfloat16* const row_max = reinterpret_cast<__nv_bfloat16*>(smem + L::kOffRow) + x * 2 * BQ + row;   // [half * BQ]
+    float* const row_max = reinterpret_cast<float*>(smem + L::kOffRow) + x * BQ + row;
     const int r = r0 + x * BQ + row;             // row of the pack
     const bool row_in = x * BQ + row < row_count, real = r < rg.n * G;
     const int qpos = real ? rg.base + r / G : -1;
@@ -446,6 +446,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const float sl = a.scale * 1.4426950408889634f;
     float m_ref = -1.0e30f, l_run = 0.0f;
     bool ok = true;
+    // Some row of the warp has a reference so large that rounding reference * sl would show (from 2^10 on by more than 2^-14 of a
+    // probability, from 2^31 on by all of it): the reference is taken from the scores before they are scaled.
+    bool far = false;
     float sv[32];
     for (int i = 0; i < n_x; ++i) {
       const int kv0 = (lo[x] + i) * BKV + half * 64;
@@ -482,7 +485,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         return fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
       };
       auto probabilities = [&](int piece) {
-        const uint64_t sl2 = pack2(sl, sl), m2 = pack2(-m_ref * sl, -m_ref * sl);
+        if (far) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) sv[e] -= m_ref;
+        }
+        const float off = far ? 0.0f : -m_ref * sl;
+        const uint64_t sl2 = pack2(sl, sl), m2 = pack2(off, off);
         uint32_t packed[16];
         uint64_t sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
@@ -506,8 +514,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       load(0);
       m_tile = largest(m_tile);
       // Both threads of a row have to use one reference. Whether any of the pair's rows wants a higher one is a barrier
-      // with a vote; only then the maxima themselves are exchanged (rounded up to bf16: all that matters is that both have
-      // the same number, within a step of the largest). The next vote keeps a next exchange behind this one's reads.
+      // with a vote; only then the maxima themselves are exchanged, in fp32 (a reference above the true maximum by as little
+      // as 2^-8 of it loses every probability of a row with large scores) through one word per row, which is all that
+      // there is room for. The next vote keeps a next exchange behind this one's reads.
       const bool raise = (m_tile - m_ref) * sl > kRescaleThreshold;
       uint32_t any_raise;
       asm volatile(
@@ -521,16 +530,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           : "r"(static_cast<uint32_t>(raise)), "r"(pair_bar)
           : "memory");
       if (any_raise) {
-        const __nv_bfloat16 up = __float2bfloat16_ru(m_tile);
-        row_max[half * BQ] = up;
+        if (half == 1) *row_max = m_tile;
         asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-        m_tile = fmaxf(__bfloat162float(up), __bfloat162float(row_max[(half ^ 1) * BQ]));
+        if (half == 0) *row_max = m_tile = fmaxf(m_tile, *row_max);
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        if (half == 1) m_tile = *row_max;
         float alpha = 1.0f;
         if ((m_tile - m_ref) * sl > kRescaleThreshold) {
           alpha = fast_exp2((m_ref - m_tile) * sl);
           m_ref = m_tile;
           l_run *= alpha;
         }
+        far = __any_sync(0xffffffffu, m_ref > -1.0e30f && fabsf(m_ref * sl) > 1024.0f);
         if (i > 0) {   // the scores of this tile came after the P V product of the one before: O is at rest
 #pragma unroll 1
           for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {

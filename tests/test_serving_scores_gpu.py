@@ -1,0 +1,46 @@
+"""Attention over the pages where scores are large, by both kernels."""
+import pytest
+import torch
+
+from nanochat_cpp_b200 import ops
+
+import serving_range_util as R
+import serving_util as U
+
+pytestmark = pytest.mark.gpu
+
+ROWS, CHUNK = R.ROWS, R.CHUNK
+
+
+@pytest.mark.parametrize("variant", [ROWS, CHUNK])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("size", [8.0, 64.0, 512.0, 8192.0, 2.0 ** 20])
+def test_one_visible_key_of_any_score(variant, mx, size):
+    """A row that sees one key gives that key's value, whatever the score (2^-8 for the probability's rounding against the sum of
+    the unrounded ones, 2^-8 for the result's)."""
+    g = torch.Generator().manual_seed(int(size) % 1000)
+    B, T, H, D = 2, 150, 3, 128
+    q, k = (torch.randn(B, T, H, D, generator=g) * size for _ in range(2))
+    c = R.case(q, k, torch.randn(B, T, H, D, generator=g), [T, T], mx)
+    out = R.run(c, variant, window=0).double()
+    v = U.pool_values(c["v"], c["vs"])[c["table"].long()].flatten(1, 2)[:, :T]
+    assert bool(((out - v).abs() <= 1.01 * 2.0 ** -7 * v.abs()).all())
+    ops.cuda_module().check_status()
+
+
+@pytest.mark.parametrize("variant", [ROWS, CHUNK])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("D,S", [(128, 700), (64, 1500)])
+def test_equal_keys_of_large_scores(variant, mx, D, S):
+    """Whole numbers: every score is exact, up to 5e4 after scaling. Keys come in a few kinds, so that many share the largest one and
+    the result is a mean of values."""
+    g = torch.Generator().manual_seed(D)
+    B, T, H, KV = 2, 90, 4, 2
+    q = torch.randint(-7, 8, (B, T, H, D), generator=g).float() * 8
+    kinds = torch.randint(-7, 8, (B, 6, KV, D), generator=g).float() * 8       # E4M3 holds 4 significant bits
+    kinds[:, 0] = q[:, 0, ::2].sign() * 56
+    k = kinds[torch.arange(B)[:, None], torch.randint(0, 6, (B, S), generator=g)]
+    c = R.case(q, k, torch.randn(B, S, KV, D, generator=g), [S, S - 41], mx)
+    R.hold(c, variant, exact_products=True)
+    R.hold(c, variant, window=300, scale=1.0, exact_products=True)
+    R.hold(c, variant, scale=64.0 * D, exact_products=True)                     # up to 2^32
