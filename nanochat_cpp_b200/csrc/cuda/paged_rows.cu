@@ -16,7 +16,9 @@
 // writes its partial sums; a combine kernel joins the runs of a row. Nothing in the CTA waits for anything else, and
 // sequences of different lengths even out over many equal units. The reference maximum of a row is raised only when a
 // score exceeds it by 2^8 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
-// Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32.
+// Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32. On MXFP8 pages
+// the products run in f16, which takes E4M3 codes in one instruction a pair and probabilities to 11 bits (and to 2^-32 of the
+// reference). A run whose blocks, or whose queries' channels, lie further apart than f16 reaches is walked again in bf16.
 // Measured (B200, MXFP8, D = 128): 64 sequences up to 2048 keys 50 us (3.45 TB/s), 32 up to 32768 172..181 us (4.9 TB/s);
 // 64 x 4 new tokens over bf16 70 us (4.9 TB/s).
 #include <cuda_bf16.h>
@@ -43,6 +45,8 @@ constexpr int kStages = 3;       // ring depth per warp
 constexpr int kMaxRun = 512;     // keys of one warp's run at most: its page numbers fit one per lane
 constexpr float kRaise = 8.0f;   // log2 units
 constexpr float kNoMax = -1.0e30f;
+constexpr int kReach = 14;       // powers of two from the largest scale to one that is a normal f16: its codes are exact there
+constexpr int kClimb = 45;       // that the scale of the values' sums may grow by before what was summed first would lose bits
 
 template <bool F16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -81,6 +85,12 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float pow2(int d) { return __uint_as_float(static_cast<uint32_t>(min(max(127 + d, 0), 255)) << 23); }
 // 2^d for d <= 0 (0 below the range of fp32)
 __device__ __forceinline__ float pow2_neg(int d) { return __uint_as_float(static_cast<uint32_t>(max(127 + d, 0)) << 23); }
+// of each half the smaller magnitude (its sign means nothing)
+__device__ __forceinline__ uint32_t min_magnitude_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -124,13 +134,13 @@ struct Ring {
   }
 };
 
-// P16: page_size is a multiple of 16, so a tile lies in one page.
-template <int D, bool MX, int NT, bool P16>
-__global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(const PagedAttnArgs a) {
+// One run of keys. P16: page_size is a multiple of 16, so a tile lies in one page. F16 (MXFP8 pages): the products run in f16, on codes
+// and powers of two, which is exact while the numbers fit it; where they do not, nothing has been written and the answer is
+// false. Without F16 they run in bf16, which holds every value of either cache.
+template <int D, bool MX, bool F16, int NT, bool P16>
+__device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
   using R = Ring<D, MX>;
   constexpr int ROWS = 8 * NT;
-  extern __shared__ __align__(16) uint8_t smem[];
-  NC_PDL_PROLOGUE();
   const int G = a.H / a.KV;
   const int lane = threadIdx.x, g8 = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.KV, rb = blockIdx.y / a.KV, b = blockIdx.z;
@@ -139,7 +149,7 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
   const int split_tiles = a.split_keys / kTile;
   const int t0 = rg.tile0 + split * split_tiles;
   const int count = min(rg.tiles - split * split_tiles, split_tiles);
-  if (split > 0 && count <= 0) return;
+  if (split > 0 && count <= 0) return true;
   if (split == 0 && lane == 0 && rg.pmax >= static_cast<long long>(a.max_pages) * a.page_size && a.status != nullptr)
     atomicCAS(a.status, 0, kErrBadIndex);   // keys past the page table are left out
   const float sl = a.scale * 1.4426950408889634f;
@@ -148,11 +158,13 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
     const int t = (r0 + r) / G, h = kvh * G + (r0 + r) % G;
     return a.q + b * a.q_stride_b + t * a.q_stride_t + h * a.q_stride_h;
   };
-  // Q as the B operand: row nt * 8 + g8, contraction step s covers channels c * D/4 + 4 s .. + 3. For MXFP8 the products
-  // run in f16, which holds E4M3 codes exactly; a row of Q is brought below 2^15 by a power of two, so that bf16's
-  // 8 bits survive down to 2^-29 of the row's largest magnitude, and the power goes into the row's score factor.
+  // Q as the B operand: row nt * 8 + g8, contraction step s covers channels c * D/4 + 4 s .. + 3. For f16 a row of Q is brought
+  // below 2^15 by a power of two, which goes into the row's score factor: exact if its smallest nonzero magnitude lies no more
+  // than 31 powers of two below the largest (bf16's 8 bits then end at f16's last step, 2^-24, or before). Rows with a
+  // result below 2^-17, zeros among them, are looked at again when the first keys have been asked for.
   uint32_t qf[NT][D / 8];
   float row_factor[NT];
+  bool tiny = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = nt * 8 + g8;
@@ -164,7 +176,7 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
       qf[nt][4 * i] = x.x, qf[nt][4 * i + 1] = x.y, qf[nt][4 * i + 2] = x.z, qf[nt][4 * i + 3] = x.w;
     }
     row_factor[nt] = sl;
-    if constexpr (MX) {
+    if constexpr (F16) {
       uint32_t mx = 0;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) mx = __vmaxu2(mx, qf[nt][i] & 0x7fff7fffu);
@@ -176,9 +188,14 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
       e = max(e, 15);
       const float up = __uint_as_float(static_cast<uint32_t>(min(127 + 14 + 127 - e, 254)) << 23);
       const float down = __uint_as_float(static_cast<uint32_t>(max(e - 14, 1)) << 23);
+      uint32_t least = 0x7c007c00u;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) qf[nt][i] = pack_f16(bf16_lo(qf[nt][i]) * up, bf16_hi(qf[nt][i]) * up);
+      for (int i = 0; i < D / 8; ++i) {
+        qf[nt][i] = pack_f16(bf16_lo(qf[nt][i]) * up, bf16_hi(qf[nt][i]) * up);
+        least = min_magnitude_f16x2(least, qf[nt][i]);
+      }
       row_factor[nt] = down * sl;
+      tiny = tiny || (ok && min(least & 0x7fffu, (least >> 16) & 0x7fffu) < 0x80u);
     }
   }
   float factor[NT][2];   // score factor of the rows this lane holds scores of (accumulator columns 2c, 2c + 1)
@@ -208,11 +225,11 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
   float l[NT][4];        // sums of the rounded probabilities: P^T times a row of ones on the tensor core
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = kNoMax, l[nt][0] = l[nt][1] = l[nt][2] = l[nt][3] = 0.0f;
-  // MXFP8: codes enter the products as code * 2^(b - ref), ref the largest scale byte of the run so far (one for keys, one
-  // for values): f16 holds that exactly as long as scales differ by no more than 2^15, and to 2^-33 of the largest
-  // beyond. The scores take 2^(k_ref - 127) into their factor; a larger v_ref scales down what has been summed.
-  int k_ref = 0, v_ref = 0;
-  float k_unit = 0.0f;
+  // Codes enter the f16 products as code * 2^(b - ref): exact while b lies no more than kReach below ref, the largest scale
+  // byte of the tile's usable keys or more (keys), of the run's usable values so far (values). The scores take 2^(k_ref - 127)
+  // into their factor; a larger v_ref scales down what has been summed.
+  int k_ref = 0, v_ref = 0, v_first = 0;
+  float k_unit = 1.0f;
 
   uint8_t* ring = smem;
   const int* table = a.page_table + static_cast<long long>(b) * a.max_pages;
@@ -322,6 +339,30 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
     if (i < count) issue(i);
     copy_commit();
   }
+  if (F16 && __any_sync(0xffffffffu, tiny)) {
+    bool lost = false;
+#pragma unroll 1
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g8;
+      const bool ok = r < row_count && (r0 + r) < rg.n * G;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(ok ? q_row(r) + c * (D / 4) : a.q);
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int i = 0; i < D / 4; ++i) top = max(top, src[i] & 0x7fffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll 1
+      for (int i = 0; i < D / 4; ++i) {
+        const uint32_t x = src[i] & 0x7fffu;
+        lost = lost || (ok && top < 0x7f80u && x != 0 && (x >> 7) + 31 < (top >> 7));
+      }
+    }
+    if (__any_sync(0xffffffffu, lost)) {
+      copy_wait<0>();
+      __syncwarp();
+      return false;
+    }
+  }
   for (int i = 0; i < count; ++i) {
     copy_wait<kStages - 2>();
     __syncwarp();    // this stage has arrived for every lane; the stage before it has been read by every lane
@@ -344,39 +385,81 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
     float s2[NT][4];   // two chains of products, added at the end
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
-    uint32_t f1[2], g1[2];   // factors of this lane's share of keys g8, g8 + 8 and of value rows (2c, 2c + 1), (2c + 8, 2c + 9)
+    // Factors of this lane's share of keys g8, g8 + 8 and of value rows (2c, 2c + 1), (2c + 8, 2c + 9); for bf16 in two steps.
+    uint32_t f1[2], g1[2], f2[2], g2[2];
     if constexpr (MX) {
       const uint8_t* sk = st + R::kOffS + g8 * (D / 32) + c * (D / 4) / 32;
       const uint8_t* sw = st + R::kOffS + R::kScale + 2 * c * (D / 32) + g8 * (D / 8) / 32;
       int bk[2] = {sk[0], sk[8 * (D / 32)]};
       int bv[4] = {sw[0], sw[D / 32], sw[8 * (D / 32)], sw[9 * (D / 32)]};
-      if (__any_sync(0xffffffffu, max(bk[0], bk[1]) > k_ref || max(max(bv[0], bv[1]), max(bv[2], bv[3])) > v_ref)) {
-        // rare: a larger scale than any so far. NaN (255: the codes are NaN already) and keys that are none count for nothing
+      if constexpr (F16) {
+        // places above the lowest scale in reach: 0 .. kReach, or anything as unsigned numbers
+        uint32_t uk[2], uv[4], most = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = 0;
+        for (int j = 0; j < 2; ++j) uk[j] = bk[j] - (k_ref - kReach), most = max(most, uk[j]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (bv[j] == 255 || !key_ok(2 * c + (j & 1) + 8 * (j >> 1))) bv[j] = 0;
-        k_ref = max(k_ref, __reduce_max_sync(0xffffffffu, max(bk[0], bk[1])));
-        k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
-        const int next = max(v_ref, __reduce_max_sync(0xffffffffu, max(max(bv[0], bv[1]), max(bv[2], bv[3]))));
-        const float alpha = pow2_neg(v_ref - next);
-        v_ref = next;
+        for (int j = 0; j < 4; ++j) uv[j] = bv[j] - (v_ref - kReach), most = max(most, uv[j]);
+        if (__any_sync(0xffffffffu, most > static_cast<uint32_t>(kReach))) {
+          // rare: other references. NaN (255: the codes are NaN already) and keys that are none count for nothing
+          int hk = 0, lk = 255, hv = 0, lv = 255;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d)
+          for (int j = 0; j < 2; ++j) {
+            if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = -1;
+            else hk = max(hk, bk[j]), lk = min(lk, bk[j]);
+          }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int j = 0; j < 4; ++j) {
+            if (bv[j] == 255 || !key_ok(2 * c + (j & 1) + 8 * (j >> 1))) bv[j] = -1;
+            else hv = max(hv, bv[j]), lv = min(lv, bv[j]);
+          }
+          hk = __reduce_max_sync(0xffffffffu, hk), lk = __reduce_min_sync(0xffffffffu, lk);
+          hv = __reduce_max_sync(0xffffffffu, hv), lv = __reduce_min_sync(0xffffffffu, lv);
+          hk = hk > 0 ? hk : k_ref, hv = max(hv, v_ref);
+          v_first = v_first > 0 ? v_first : hv;
+          if (lk < hk - kReach || lv < hv - kReach || hv - v_first > kClimb) {   // too far apart for f16
+            copy_wait<0>();
+            __syncwarp();
+            return false;
+          }
+          k_ref = hk, k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
+          const float alpha = pow2_neg(v_ref - hv);
+          v_ref = hv;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[d][nt][e] *= alpha;
-      }
+          for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float f = pow2_neg(bk[j] - k_ref);
-        f1[j] = pack_f16(f, f);
-        g1[j] = pack_f16(pow2_neg(bv[2 * j] - v_ref), pow2_neg(bv[2 * j + 1] - v_ref));
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[d][nt][e] *= alpha;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) uk[j] = bk[j] < 0 ? kReach : bk[j] - (k_ref - kReach);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) uv[j] = bv[j] < 0 ? kReach : bv[j] - (v_ref - kReach);
+        }
+        // 2^(u - kReach) as f16: the exponent field is u + 1
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          f1[j] = uk[j] * 0x04000400u + 0x04000400u;
+          g1[j] = uv[2 * j] * 0x400u + uv[2 * j + 1] * 0x04000000u + 0x04000400u;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k0 = 2 * c + 8 * j;
+          const uint32_t b = key_ok(g8 + 8 * j) ? bk[j] : 127, b0 = key_ok(k0) ? bv[2 * j] : 127, b1 = key_ok(k0 + 1) ? bv[2 * j + 1] : 127;
+          f1[j] = mx_factor_first(b) * 0x10001u, f2[j] = mx_factor_second(b) * 0x10001u;
+          g1[j] = mx_factor_first(b0) | mx_factor_first(b1) << 16, g2[j] = mx_factor_second(b0) | mx_factor_second(b1) << 16;
+        }
       }
     }
+    // four codes -> two registers of an operand, scaled
+    auto scaled = [&](uint32_t w, uint32_t first, uint32_t second, uint32_t& lo, uint32_t& hi) {
+      if constexpr (F16) {
+        lo = mul_f16x2(codes_lo(w), first), hi = mul_f16x2(codes_hi(w), first);
+      } else {
+        mx_spread(w, lo, hi);
+        lo = mul_bf16x2(mul_bf16x2(lo, first), second), hi = mul_bf16x2(mul_bf16x2(hi, first), second);
+      }
+    };
 #pragma unroll
     for (int x = 0; x < R::kRow / 64; ++x) {
       const uint4 w0 = *reinterpret_cast<const uint4*>(st + k_at[x]);
@@ -385,10 +468,11 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
       if constexpr (MX) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const uint32_t fa[4] = {mul_f16x2(codes_lo(u0[y]), f1[0]), mul_f16x2(codes_lo(u1[y]), f1[1]),
-                                  mul_f16x2(codes_hi(u0[y]), f1[0]), mul_f16x2(codes_hi(u1[y]), f1[1])};
+          uint32_t fa[4];
+          scaled(u0[y], f1[0], f2[0], fa[0], fa[2]);
+          scaled(u1[y], f1[1], f2[1], fa[1], fa[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<true>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
         }
       } else {
 #pragma unroll
@@ -402,7 +486,7 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (MX ? factor[nt][e & 1] * k_unit : factor[nt][e & 1]);
+      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (F16 ? factor[nt][e & 1] * k_unit : factor[nt][e & 1]);
 
     // ---- masks, running maximum, probabilities
     if (edge) {
@@ -437,15 +521,16 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
     uint32_t pf[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      // f16 probabilities are taken 2^7 times too large (below 2^15): small ones keep their bits; the sums carry the factor too
+      // f16 probabilities are taken 2^7 times too large (below 2^15): small ones keep their bits; the sums carry the factor too,
+      // and so do those of runs in bf16, which are joined with them
       const float c0 = m[nt][0] - (MX ? 7.0f : 0.0f), c1 = m[nt][1] - (MX ? 7.0f : 0.0f);
       const float p0 = fast_exp2(s[nt][0] - c0), p1 = fast_exp2(s[nt][1] - c1);
       const float p2 = fast_exp2(s[nt][2] - c0), p3 = fast_exp2(s[nt][3] - c1);
-      pf[nt][0] = transpose_8x8(MX ? pack_f16(p0, p1) : pack_bf16(p0, p1));
-      pf[nt][1] = transpose_8x8(MX ? pack_f16(p2, p3) : pack_bf16(p2, p3));
-      constexpr uint32_t kOne = MX ? 0x3c003c00u : 0x3f803f80u;
+      pf[nt][0] = transpose_8x8(F16 ? pack_f16(p0, p1) : pack_bf16(p0, p1));
+      pf[nt][1] = transpose_8x8(F16 ? pack_f16(p2, p3) : pack_bf16(p2, p3));
+      constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
       const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-      mma_16816<MX>(l[nt], ones, pf[nt][0], pf[nt][1]);
+      mma_16816<F16>(l[nt], ones, pf[nt][0], pf[nt][1]);
     }
 
     // ---- O^T += V^T P^T: keys 2c, 2c + 1 (low, high half of a register) and 2c + 8, 2c + 9
@@ -468,14 +553,14 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t ab = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x5140), cd = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x7362);
-          f[j][0] = mul_f16x2(codes_lo(ab), g1[j]), f[j][1] = mul_f16x2(codes_hi(ab), g1[j]);
-          f[j][2] = mul_f16x2(codes_lo(cd), g1[j]), f[j][3] = mul_f16x2(codes_hi(cd), g1[j]);
+          scaled(ab, g1[j], g2[j], f[j][0], f[j][1]);
+          scaled(cd, g1[j], g2[j], f[j][2], f[j][3]);
         }
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const uint32_t fa[4] = {f[0][2 * z], f[0][2 * z + 1], f[1][2 * z], f[1][2 * z + 1]};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<true>(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
         }
       }
     } else {
@@ -499,7 +584,7 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
 
   // ---- the run's result: rows 2c, 2c + 1 of every eight, channels g8 * D/8 + x
   const bool whole = rg.tiles <= split_tiles;   // no other run has keys: the result is final
-  const float unit = MX ? pow2(v_ref - 127) : 1.0f;
+  const float unit = F16 ? pow2(v_ref - 127) : 1.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -532,6 +617,22 @@ __global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(
         if (g8 == 0) *reinterpret_cast<float2*>(a.part_ml + (at * rw + r) * 2) = make_float2(m[nt][e], sum);
       }
     }
+  return true;
+}
+
+// A function of its own, so that what f16 cannot hold takes no registers from what it can.
+template <int D, int NT, bool P16>
+__device__ __noinline__ void walk_in_bf16(const PagedAttnArgs& a, uint8_t* smem) {
+  walk<D, true, false, NT, P16>(a, smem);
+}
+
+template <int D, bool MX, int NT, bool P16>
+__global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  NC_PDL_PROLOGUE();
+  if (!walk<D, MX, MX, NT, P16>(a, smem)) {
+    if constexpr (MX) walk_in_bf16<D, NT, P16>(a, smem);
+  }
 }
 
 // Rows per CTA: the query rows of a kv head in blocks of 8, 16 or 32.
