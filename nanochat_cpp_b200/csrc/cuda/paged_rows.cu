@@ -15,7 +15,7 @@
 // A warp is a unit of its own: it takes one run of keys (`split_keys`) of one sequence, kv head and block of rows, and
 // writes its partial sums; a combine kernel joins the runs of a row. Nothing in the CTA waits for anything else, and
 // sequences of different lengths even out over many equal units. The reference maximum of a row is raised only when a
-// score exceeds it by 2^8 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
+// score exceeds it by 2^8 or 2^7 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
 // Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32. On MXFP8 pages
 // the products run in f16, which takes E4M3 codes in one instruction a pair and probabilities to 11 bits (and to 2^-32 of the
 // reference). A run whose blocks, or whose queries' channels, lie further apart than f16 reaches is walked again in bf16.
@@ -43,7 +43,6 @@ namespace {
 constexpr int kTile = 16;        // keys per warp step
 constexpr int kStages = 3;       // ring depth per warp
 constexpr int kMaxRun = 512;     // keys of one warp's run at most: its page numbers fit one per lane
-constexpr float kRaise = 8.0f;   // log2 units
 constexpr float kNoMax = -1.0e30f;
 constexpr int kReach = 14;       // powers of two from the largest scale to one that is a normal f16: its codes are exact there
 constexpr int kClimb = 45;       // that the scale of the values' sums may grow by before what was summed first would lose bits
@@ -141,6 +140,9 @@ template <int D, bool MX, bool F16, int NT, bool P16>
 __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
   using R = Ring<D, MX>;
   constexpr int ROWS = 8 * NT;
+  // By how much a score may exceed its row's reference, in log2 units. In f16 (below 2^16) probabilities are taken 2^7 times too large,
+  // and where scores are so large that fp32 steps by 8, "7 below the reference" is 8 below it: 2^15 at most.
+  constexpr float kRaise = F16 ? 7.0f : 8.0f;
   const int G = a.H / a.KV;
   const int lane = threadIdx.x, g8 = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y % a.KV, rb = blockIdx.y / a.KV, b = blockIdx.z;

@@ -44,3 +44,28 @@ def test_equal_keys_of_large_scores(variant, mx, D, S):
     R.hold(c, variant, exact_products=True)
     R.hold(c, variant, window=300, scale=1.0, exact_products=True)
     R.hold(c, variant, scale=64.0 * D, exact_products=True)                     # up to 2^32
+
+
+@pytest.mark.parametrize("variant", [ROWS, CHUNK])
+@pytest.mark.parametrize("mx", [False, True])
+def test_scores_where_fp32_steps_by_eight(variant, mx):
+    """Whole-number scores above 2^23, scaled to above 2^26 in powers of two, where fp32 holds every eighth number: the later keys'
+    scores are one step (2^8 in probability) above the first ones', so their values' mean is the result but for one part in 257."""
+    D, n = 128, 16
+    q = torch.full((1, 1, 1, D), 256.0)
+    k = torch.full((1, 2 * n, 1, D), 256.0)
+    q[..., 0] = 1
+    k[..., 1:17] = 288
+    k[:, :n, :, 0], k[:, n:, :, 0] = 1, 2
+    scale = 8 / 1.4426950408889634
+    s = (k[0, :, 0] @ q[0, 0, 0]).double()
+    assert s.min() > 2 ** 23 and s[-1] - s[0] == 1
+    steps = (s.float() * (torch.tensor(scale) * 1.4426950408889634)).double()
+    assert steps.min() > 2 ** 26 and steps[-1] - steps[0] == 8
+    v = torch.randn(1, 2 * n, 1, D, generator=torch.Generator().manual_seed(1))
+    c = R.case(q, k, v, [2 * n], mx)
+    out = R.run(c, variant, scale=scale).double()[0, 0, 0]
+    values = U.pool_values(c["v"], c["vs"])[c["table"].long()].flatten(1, 2)[0, :2 * n, 0]
+    low, high = values[:n].mean(0), values[n:].mean(0)
+    assert bool(((out - (low + 256 * high) / 257).abs() <= 1.01 * 2.0 ** -7 * values.abs().mean(0) * 2).all())
+    ops.cuda_module().check_status()
