@@ -324,6 +324,7 @@ class InferenceEngine:
         self._graph = None
         self._graph_key = None
         self._graph_cache = None   # strong reference: the captured graph addresses this cache's tensors
+        self._graph_rope = None    # and the rotary tables that it was captured with, which a longer cache replaces
 
     # ------------------------------------------------------------------ helpers
     def new_cache(self, batch: int, max_seq: int) -> PagedKVCache:
@@ -637,7 +638,7 @@ class InferenceEngine:
         # compares by identity: an `id()` can be reused by a new cache once the old one is freed.
         key = (tokens.shape[0], cache.max_seq, bool(greedy))
         if self._graph_cache is not cache or self._graph_key != key:
-            self._graph = None
+            self._graph = self._graph_rope = None
             self._graph_key = key
             self._graph_cache = cache
             lens_host = list(cache.lens_host)
@@ -664,10 +665,12 @@ class InferenceEngine:
                 cache.has_prev = had
                 cache.lens_host[:] = lens_host
                 self._graph = g
+                self._graph_rope = (self._cos, self._sin)
             except Exception:
                 cache.lens_host[:] = lens_host
                 self._graph = None
                 self._graph_cache = None
+                self._graph_rope = None
                 self.use_cuda_graph = False
                 torch.cuda.synchronize()
                 return self.decode(cache, tokens, greedy)
