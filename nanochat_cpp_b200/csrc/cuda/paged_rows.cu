@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "host_build.h"
 #include "mx_cache.cuh"
@@ -42,7 +43,7 @@ namespace {
 
 constexpr int kTile = 16;        // keys per warp step
 constexpr int kStages = 3;       // ring depth per warp
-constexpr int kMaxRun = 512;     // keys of one warp's run at most: its page numbers fit one per lane
+constexpr int kPart = 512;       // keys of a run whose page numbers are at hand, one per lane: a longer run goes part by part
 constexpr float kNoMax = -1.0e30f;
 constexpr int kReach = 14;       // powers of two from the largest scale to one that is a normal f16: its codes are exact there
 constexpr int kClimb = 45;       // that the scale of the values' sums may grow by before what was summed first would lose bits
@@ -149,9 +150,9 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
   const int r0 = rb * ROWS, row_count = min(ROWS, a.T * G - r0);
   const Range rg = range_of(a, b, r0, ROWS, kTile);
   const int split_tiles = a.split_keys / kTile;
-  const int t0 = rg.tile0 + split * split_tiles;
-  const int count = min(rg.tiles - split * split_tiles, split_tiles);
-  if (split > 0 && count <= 0) return true;
+  int t0 = rg.tile0 + split * split_tiles, left = min(rg.tiles - split * split_tiles, split_tiles);
+  if (split > 0 && left <= 0) return true;
+  int count = min(left, kPart / kTile);   // tiles of the part that begins at tile t0
   if (split == 0 && lane == 0 && rg.pmax >= static_cast<long long>(a.max_pages) * a.page_size && a.status != nullptr)
     atomicCAS(a.status, 0, kErrBadIndex);   // keys past the page table are left out
   const float sl = a.scale * 1.4426950408889634f;
@@ -251,18 +252,19 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
   } else {
     v_at[0] = R::kOffV + 2 * c * R::kRow + R::place_v(2 * c, g8 / 2) * 16 + (g8 & 1) * 8;
   }
-  // P16: lane i holds the i-th page of the run, and `at_page`, `in_page` follow the tiles that are requested
+  // P16: lane i holds the i-th page of the part, and `at_page`, `in_page` follow the tiles that are requested
   const int tiles_per_page = P16 ? a.page_size / kTile : 1;
   int page_ids = -1, at_page = 0, in_page = 0;
   unsigned bad_tiles = 0;   // P16: bit i: the page of tile i is unmapped or outside the pool
-  if constexpr (P16) {
+  auto look_up = [&]() {
     const int first = t0 / tiles_per_page;
-    in_page = t0 - first * tiles_per_page;
+    at_page = 0, in_page = t0 - first * tiles_per_page, page_ids = -1;
     if (count > 0 && first + lane <= (t0 + count - 1) / tiles_per_page) page_ids = table[first + lane];
     const int mine = __shfl_sync(0xffffffffu, page_ids, (in_page + lane) / tiles_per_page);
     bad_tiles = __ballot_sync(0xffffffffu, lane < count && (mine < 0 || mine >= a.num_pages));
     if (bad_tiles != 0 && lane == 0 && a.status != nullptr) atomicCAS(a.status, 0, kErrBadIndex);
-  }
+  };
+  if constexpr (P16) look_up();
   const uint8_t* s_lane = nullptr;
   uint32_t s_dst = 0, s_stride = 0;
   constexpr int kScaleLanes = MX ? R::kScale / 16 : 1;   // 16-byte pieces of a tile's scales, one side
@@ -336,11 +338,14 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
     }
   };
 
+  auto begin = [&]() {
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (i < count) issue(i);
-    copy_commit();
-  }
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < count) issue(i);
+      copy_commit();
+    }
+  };
+  begin();
   if (F16 && __any_sync(0xffffffffu, tiny)) {
     bool lost = false;
 #pragma unroll 1
@@ -365,222 +370,231 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
       return false;
     }
   }
-  for (int i = 0; i < count; ++i) {
-    copy_wait<kStages - 2>();
-    __syncwarp();    // this stage has arrived for every lane; the stage before it has been read by every lane
-    if (i + kStages - 1 < count) issue(i + kStages - 1);
-    copy_commit();
-    const uint8_t* st = ring + get * R::kStage;
-    get = get + 1 == kStages ? 0 : get + 1;
-    const int key0 = (t0 + i) * kTile;
-    const int page_info = P16 ? 0 : *reinterpret_cast<const int*>(st + R::kOffPage);
-    const bool tile_ok = P16 ? ((bad_tiles >> i) & 1) == 0 : page_info == 0xffff;
-    const bool edge = key0 < all_lo || key0 + kTile > all_hi || !tile_ok;
-    auto key_ok = [&](int k) {   // key0 + k holds a key of the cache that some row may see
-      return key0 + k >= rg.lo && key0 + k < rg.hi && (P16 ? tile_ok : ((page_info >> k) & 1) != 0);
-    };
+  while (true) {
+    for (int i = 0; i < count; ++i) {
+      copy_wait<kStages - 2>();
+      __syncwarp();    // this stage has arrived for every lane; the stage before it has been read by every lane
+      if (i + kStages - 1 < count) issue(i + kStages - 1);
+      copy_commit();
+      const uint8_t* st = ring + get * R::kStage;
+      get = get + 1 == kStages ? 0 : get + 1;
+      const int key0 = (t0 + i) * kTile;
+      const int page_info = P16 ? 0 : *reinterpret_cast<const int*>(st + R::kOffPage);
+      const bool tile_ok = P16 ? ((bad_tiles >> i) & 1) == 0 : page_info == 0xffff;
+      const bool edge = key0 < all_lo || key0 + kTile > all_hi || !tile_ok;
+      auto key_ok = [&](int k) {   // key0 + k holds a key of the cache that some row may see
+        return key0 + k >= rg.lo && key0 + k < rg.hi && (P16 ? tile_ok : ((page_info >> k) & 1) != 0);
+      };
 
-    // ---- S^T = K Q^T
-    float s[NT][4];
+      // ---- S^T = K Q^T
+      float s[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-    float s2[NT][4];   // two chains of products, added at the end
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+      float s2[NT][4];   // two chains of products, added at the end
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
-    // Factors of this lane's share of keys g8, g8 + 8 and of value rows (2c, 2c + 1), (2c + 8, 2c + 9); for bf16 in two steps.
-    uint32_t f1[2], g1[2], f2[2], g2[2];
-    if constexpr (MX) {
-      const uint8_t* sk = st + R::kOffS + g8 * (D / 32) + c * (D / 4) / 32;
-      const uint8_t* sw = st + R::kOffS + R::kScale + 2 * c * (D / 32) + g8 * (D / 8) / 32;
-      int bk[2] = {sk[0], sk[8 * (D / 32)]};
-      int bv[4] = {sw[0], sw[D / 32], sw[8 * (D / 32)], sw[9 * (D / 32)]};
-      if constexpr (F16) {
-        // places above the lowest scale in reach: 0 .. kReach, or anything as unsigned numbers
-        uint32_t uk[2], uv[4], most = 0;
+      for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.0f;
+      // Factors of this lane's share of keys g8, g8 + 8 and of value rows (2c, 2c + 1), (2c + 8, 2c + 9); for bf16 in two steps.
+      uint32_t f1[2], g1[2], f2[2], g2[2];
+      if constexpr (MX) {
+        const uint8_t* sk = st + R::kOffS + g8 * (D / 32) + c * (D / 4) / 32;
+        const uint8_t* sw = st + R::kOffS + R::kScale + 2 * c * (D / 32) + g8 * (D / 8) / 32;
+        int bk[2] = {sk[0], sk[8 * (D / 32)]};
+        int bv[4] = {sw[0], sw[D / 32], sw[8 * (D / 32)], sw[9 * (D / 32)]};
+        if constexpr (F16) {
+          // places above the lowest scale in reach: 0 .. kReach, or anything as unsigned numbers
+          uint32_t uk[2], uv[4], most = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) uk[j] = bk[j] - (k_ref - kReach), most = max(most, uk[j]);
+          for (int j = 0; j < 2; ++j) uk[j] = bk[j] - (k_ref - kReach), most = max(most, uk[j]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) uv[j] = bv[j] - (v_ref - kReach), most = max(most, uv[j]);
-        if (__any_sync(0xffffffffu, most > static_cast<uint32_t>(kReach))) {
-          // rare: other references. NaN (255: the codes are NaN already) and keys that are none count for nothing
-          int hk = 0, lk = 255, hv = 0, lv = 255;
+          for (int j = 0; j < 4; ++j) uv[j] = bv[j] - (v_ref - kReach), most = max(most, uv[j]);
+          if (__any_sync(0xffffffffu, most > static_cast<uint32_t>(kReach))) {
+            // rare: other references. NaN (255: the codes are NaN already) and keys that are none count for nothing
+            int hk = 0, lk = 255, hv = 0, lv = 255;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = -1;
+              else hk = max(hk, bk[j]), lk = min(lk, bk[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (bv[j] == 255 || !key_ok(2 * c + (j & 1) + 8 * (j >> 1))) bv[j] = -1;
+              else hv = max(hv, bv[j]), lv = min(lv, bv[j]);
+            }
+            hk = __reduce_max_sync(0xffffffffu, hk), lk = __reduce_min_sync(0xffffffffu, lk);
+            hv = __reduce_max_sync(0xffffffffu, hv), lv = __reduce_min_sync(0xffffffffu, lv);
+            hk = hk > 0 ? hk : k_ref, hv = max(hv, v_ref);
+            v_first = v_first > 0 ? v_first : hv;
+            if (lk < hk - kReach || lv < hv - kReach || hv - v_first > kClimb) {   // too far apart for f16
+              copy_wait<0>();
+              __syncwarp();
+              return false;
+            }
+            k_ref = hk, k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
+            const float alpha = pow2_neg(v_ref - hv);
+            v_ref = hv;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[d][nt][e] *= alpha;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) uk[j] = bk[j] < 0 ? kReach : bk[j] - (k_ref - kReach);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) uv[j] = bv[j] < 0 ? kReach : bv[j] - (v_ref - kReach);
+          }
+          // 2^(u - kReach) as f16: the exponent field is u + 1
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = -1;
-            else hk = max(hk, bk[j]), lk = min(lk, bk[j]);
+            f1[j] = uk[j] * 0x04000400u + 0x04000400u;
+            g1[j] = uv[2 * j] * 0x400u + uv[2 * j + 1] * 0x04000000u + 0x04000400u;
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (bv[j] == 255 || !key_ok(2 * c + (j & 1) + 8 * (j >> 1))) bv[j] = -1;
-            else hv = max(hv, bv[j]), lv = min(lv, bv[j]);
-          }
-          hk = __reduce_max_sync(0xffffffffu, hk), lk = __reduce_min_sync(0xffffffffu, lk);
-          hv = __reduce_max_sync(0xffffffffu, hv), lv = __reduce_min_sync(0xffffffffu, lv);
-          hk = hk > 0 ? hk : k_ref, hv = max(hv, v_ref);
-          v_first = v_first > 0 ? v_first : hv;
-          if (lk < hk - kReach || lv < hv - kReach || hv - v_first > kClimb) {   // too far apart for f16
-            copy_wait<0>();
-            __syncwarp();
-            return false;
-          }
-          k_ref = hk, k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
-          const float alpha = pow2_neg(v_ref - hv);
-          v_ref = hv;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[d][nt][e] *= alpha;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) uk[j] = bk[j] < 0 ? kReach : bk[j] - (k_ref - kReach);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) uv[j] = bv[j] < 0 ? kReach : bv[j] - (v_ref - kReach);
-        }
-        // 2^(u - kReach) as f16: the exponent field is u + 1
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          f1[j] = uk[j] * 0x04000400u + 0x04000400u;
-          g1[j] = uv[2 * j] * 0x400u + uv[2 * j + 1] * 0x04000000u + 0x04000400u;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int k0 = 2 * c + 8 * j;
-          const uint32_t b = key_ok(g8 + 8 * j) ? bk[j] : 127, b0 = key_ok(k0) ? bv[2 * j] : 127, b1 = key_ok(k0 + 1) ? bv[2 * j + 1] : 127;
-          f1[j] = mx_factor_first(b) * 0x10001u, f2[j] = mx_factor_second(b) * 0x10001u;
-          g1[j] = mx_factor_first(b0) | mx_factor_first(b1) << 16, g2[j] = mx_factor_second(b0) | mx_factor_second(b1) << 16;
-        }
-      }
-    }
-    // four codes -> two registers of an operand, scaled
-    auto scaled = [&](uint32_t w, uint32_t first, uint32_t second, uint32_t& lo, uint32_t& hi) {
-      if constexpr (F16) {
-        lo = mul_f16x2(codes_lo(w), first), hi = mul_f16x2(codes_hi(w), first);
-      } else {
-        mx_spread(w, lo, hi);
-        lo = mul_bf16x2(mul_bf16x2(lo, first), second), hi = mul_bf16x2(mul_bf16x2(hi, first), second);
-      }
-    };
-#pragma unroll
-    for (int x = 0; x < R::kRow / 64; ++x) {
-      const uint4 w0 = *reinterpret_cast<const uint4*>(st + k_at[x]);
-      const uint4 w1 = *reinterpret_cast<const uint4*>(st + k_at[x] + 8 * R::kRow);
-      const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
-      if constexpr (MX) {
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          uint32_t fa[4];
-          scaled(u0[y], f1[0], f2[0], fa[0], fa[2]);
-          scaled(u1[y], f1[1], f2[1], fa[1], fa[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t fa[4] = {u0[2 * y], u1[2 * y], u0[2 * y + 1], u1[2 * y + 1]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (2 * x + y)], qf[nt][2 * (2 * x + y) + 1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (F16 ? factor[nt][e & 1] * k_unit : factor[nt][e & 1]);
-
-    // ---- masks, running maximum, probabilities
-    if (edge) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = g8 + (e >> 1) * 8, d = pos[nt][e & 1] - (key0 + k);
-          if (!(key_ok(k) && d >= 0 && (a.window_left < 0 || d <= a.window_left))) s[nt][e] = -CUDART_INF_F;
-        }
-    }
-    bool raise = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) raise = raise || s[nt][e] - m[nt][e & 1] > kRaise;
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][e + 2]));
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float alpha = fast_exp2(m[nt][e] - mx);
-          m[nt][e] = mx;
-          l[nt][e] *= alpha, l[nt][e + 2] *= alpha;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) acc[d][nt][e] *= alpha, acc[d][nt][e + 2] *= alpha;
-        }
-    }
-    uint32_t pf[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      // f16 probabilities are taken 2^7 times too large (below 2^15): small ones keep their bits; the sums carry the factor too,
-      // and so do those of runs in bf16, which are joined with them
-      const float c0 = m[nt][0] - (MX ? 7.0f : 0.0f), c1 = m[nt][1] - (MX ? 7.0f : 0.0f);
-      const float p0 = fast_exp2(s[nt][0] - c0), p1 = fast_exp2(s[nt][1] - c1);
-      const float p2 = fast_exp2(s[nt][2] - c0), p3 = fast_exp2(s[nt][3] - c1);
-      pf[nt][0] = transpose_8x8(F16 ? pack_f16(p0, p1) : pack_bf16(p0, p1));
-      pf[nt][1] = transpose_8x8(F16 ? pack_f16(p2, p3) : pack_bf16(p2, p3));
-      constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
-      const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
-      mma_16816<F16>(l[nt], ones, pf[nt][0], pf[nt][1]);
-    }
-
-    // ---- O^T += V^T P^T: keys 2c, 2c + 1 (low, high half of a register) and 2c + 8, 2c + 9
-    if constexpr (MX) {
-      constexpr int kWords = R::kRow / 32;
-      uint32_t v[4][kWords];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kWords == 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
-          v[j][0] = w.x, v[j][1] = w.y, v[j][2] = w.z, v[j][3] = w.w;
         } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
-          v[j][0] = w.x, v[j][1] = w.y;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int k0 = 2 * c + 8 * j;
+            const uint32_t b = key_ok(g8 + 8 * j) ? bk[j] : 127, b0 = key_ok(k0) ? bv[2 * j] : 127, b1 = key_ok(k0 + 1) ? bv[2 * j + 1] : 127;
+            f1[j] = mx_factor_first(b) * 0x10001u, f2[j] = mx_factor_second(b) * 0x10001u;
+            g1[j] = mx_factor_first(b0) | mx_factor_first(b1) << 16, g2[j] = mx_factor_second(b0) | mx_factor_second(b1) << 16;
+          }
+        }
+      }
+      // four codes -> two registers of an operand, scaled
+      auto scaled = [&](uint32_t w, uint32_t first, uint32_t second, uint32_t& lo, uint32_t& hi) {
+        if constexpr (F16) {
+          lo = mul_f16x2(codes_lo(w), first), hi = mul_f16x2(codes_hi(w), first);
+        } else {
+          mx_spread(w, lo, hi);
+          lo = mul_bf16x2(mul_bf16x2(lo, first), second), hi = mul_bf16x2(mul_bf16x2(hi, first), second);
+        }
+      };
+#pragma unroll
+      for (int x = 0; x < R::kRow / 64; ++x) {
+        const uint4 w0 = *reinterpret_cast<const uint4*>(st + k_at[x]);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(st + k_at[x] + 8 * R::kRow);
+        const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+        if constexpr (MX) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            uint32_t fa[4];
+            scaled(u0[y], f1[0], f2[0], fa[0], fa[2]);
+            scaled(u1[y], f1[1], f2[1], fa[1], fa[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (4 * x + y)], qf[nt][2 * (4 * x + y) + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t fa[4] = {u0[2 * y], u1[2 * y], u0[2 * y + 1], u1[2 * y + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<false>(y & 1 ? s2[nt] : s[nt], fa, qf[nt][2 * (2 * x + y)], qf[nt][2 * (2 * x + y) + 1]);
+          }
         }
       }
 #pragma unroll
-      for (int y = 0; y < kWords; ++y) {
-        uint32_t f[2][4];   // [key pair][channel 4y + .], each (first key, second key)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t ab = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x5140), cd = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x7362);
-          scaled(ab, g1[j], g2[j], f[j][0], f[j][1]);
-          scaled(cd, g1[j], g2[j], f[j][2], f[j][3]);
-        }
+        for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (F16 ? factor[nt][e & 1] * k_unit : factor[nt][e & 1]);
+
+      // ---- masks, running maximum, probabilities
+      if (edge) {
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const uint32_t fa[4] = {f[0][2 * z], f[0][2 * z + 1], f[1][2 * z], f[1][2 * z + 1]};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int k = g8 + (e >> 1) * 8, d = pos[nt][e & 1] - (key0 + k);
+            if (!(key_ok(k) && d >= 0 && (a.window_left < 0 || d <= a.window_left))) s[nt][e] = -CUDART_INF_F;
+          }
       }
-    } else {
+      bool raise = false;
 #pragma unroll
-      for (int x = 0; x < R::kRow / 128; ++x) {
-        uint4 w[4];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(st + v_at[x] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
+        for (int e = 0; e < 4; ++e) raise = raise || s[nt][e] - m[nt][e & 1] > kRaise;
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint32_t v0 = (&w[0].x)[y], v1 = (&w[1].x)[y], v2 = (&w[2].x)[y], v3 = (&w[3].x)[y];
-          const uint32_t fa[4] = {__byte_perm(v0, v1, 0x5410), __byte_perm(v0, v1, 0x7632), __byte_perm(v2, v3, 0x5410),
-                                  __byte_perm(v2, v3, 0x7632)};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(acc[4 * x + y][nt], fa, pf[nt][0], pf[nt][1]);
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][e + 2]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float alpha = fast_exp2(m[nt][e] - mx);
+            m[nt][e] = mx;
+            l[nt][e] *= alpha, l[nt][e + 2] *= alpha;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) acc[d][nt][e] *= alpha, acc[d][nt][e + 2] *= alpha;
+          }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // f16 probabilities are taken 2^7 times too large (below 2^15): small ones keep their bits; the sums carry the factor too,
+        // and so do those of runs in bf16, which are joined with them
+        const float c0 = m[nt][0] - (MX ? 7.0f : 0.0f), c1 = m[nt][1] - (MX ? 7.0f : 0.0f);
+        const float p0 = fast_exp2(s[nt][0] - c0), p1 = fast_exp2(s[nt][1] - c1);
+        const float p2 = fast_exp2(s[nt][2] - c0), p3 = fast_exp2(s[nt][3] - c1);
+        pf[nt][0] = transpose_8x8(F16 ? pack_f16(p0, p1) : pack_bf16(p0, p1));
+        pf[nt][1] = transpose_8x8(F16 ? pack_f16(p2, p3) : pack_bf16(p2, p3));
+        constexpr uint32_t kOne = F16 ? 0x3c003c00u : 0x3f803f80u;
+        const uint32_t ones[4] = {kOne, kOne, kOne, kOne};
+        mma_16816<F16>(l[nt], ones, pf[nt][0], pf[nt][1]);
+      }
+
+      // ---- O^T += V^T P^T: keys 2c, 2c + 1 (low, high half of a register) and 2c + 8, 2c + 9
+      if constexpr (MX) {
+        constexpr int kWords = R::kRow / 32;
+        uint32_t v[4][kWords];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kWords == 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
+            v[j][0] = w.x, v[j][1] = w.y, v[j][2] = w.z, v[j][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(st + v_at[0] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
+            v[j][0] = w.x, v[j][1] = w.y;
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < kWords; ++y) {
+          uint32_t f[2][4];   // [key pair][channel 4y + .], each (first key, second key)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t ab = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x5140), cd = __byte_perm(v[2 * j][y], v[2 * j + 1][y], 0x7362);
+            scaled(ab, g1[j], g2[j], f[j][0], f[j][1]);
+            scaled(cd, g1[j], g2[j], f[j][2], f[j][3]);
+          }
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t fa[4] = {f[0][2 * z], f[0][2 * z + 1], f[1][2 * z], f[1][2 * z + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(acc[2 * y + z][nt], fa, pf[nt][0], pf[nt][1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < R::kRow / 128; ++x) {
+          uint4 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(st + v_at[x] + ((j & 1) + 8 * (j >> 1)) * R::kRow);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t v0 = (&w[0].x)[y], v1 = (&w[1].x)[y], v2 = (&w[2].x)[y], v3 = (&w[3].x)[y];
+            const uint32_t fa[4] = {__byte_perm(v0, v1, 0x5410), __byte_perm(v0, v1, 0x7632), __byte_perm(v2, v3, 0x5410),
+                                    __byte_perm(v2, v3, 0x7632)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<false>(acc[4 * x + y][nt], fa, pf[nt][0], pf[nt][1]);
+          }
         }
       }
     }
+    left -= count;
+    if (left <= 0) break;
+    copy_wait<0>();
+    __syncwarp();
+    t0 += count, count = min(left, kPart / kTile);
+    if constexpr (P16) look_up();
+    begin();
   }
   copy_wait<0>();
 
@@ -629,7 +643,7 @@ __device__ __noinline__ void walk_in_bf16(const PagedAttnArgs& a, uint8_t* smem)
 }
 
 template <int D, bool MX, int NT, bool P16>
-__global__ void __launch_bounds__(32, MX && NT == 1 ? 16 : 8) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(32, NT > 1 ? 8 : MX ? 16 : 12) paged_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   NC_PDL_PROLOGUE();
   if (!walk<D, MX, MX, NT, P16>(a, smem)) {
@@ -684,14 +698,18 @@ bool paged_rows_can(const PagedAttnArgs& a) {
 
 PagedPlan paged_rows_plan(const PagedAttnArgs& a) {
   const int G = a.H / a.KV, rows = 8 * row_tiles(a), blocks = (a.T * G + rows - 1) / rows;
-  long long keys = static_cast<long long>(a.max_pages) * a.page_size;
+  long long keys = std::min(static_cast<long long>(a.max_pages) * a.page_size, (1LL << 31) - kTile);   // lengths are ints
   if (a.window_left >= 0) keys = std::min(keys, static_cast<long long>(a.window_left) + 1 + (rows + G - 1) / G);
   const long long units = static_cast<long long>(a.B) * a.KV * blocks;
   // Runs that fill the warps of two CTAs per SM about three times over (so that the last ones even out), of 64 keys at
-  // least (below that the fixed cost of a run and of joining it outweighs the keys) and kMaxRun at most.
+  // least (below that the fixed cost of a run and of joining it outweighs the keys) and 512 at most, unless that makes more than
+  // twice as many: the runs, and with them the workspace (32 rows of D + 2 numbers each at most), are bounded. Units that
+  // are enough by themselves are not split.
   const long long want = 148LL * 16 * 3;
-  long long per = (keys * units + want - 1) / want;
-  per = (std::min<long long>(std::max<long long>(per, 64), kMaxRun) + kTile - 1) / kTile * kTile;
+  const auto share = [&](long long runs) { return static_cast<long long>(std::ceil(static_cast<double>(keys) * units / runs)); };
+  long long per = std::max(std::min<long long>(std::max<long long>(share(want), 64), 512), share(2 * want));
+  if (units >= want) per = keys;
+  per = (std::min<long long>(std::max<long long>(per, kTile), 1 << 30) + kTile - 1) / kTile * kTile;
   PagedPlan p;
   p.split_keys = static_cast<int>(per);
   // a window may start inside a tile and touch one more
