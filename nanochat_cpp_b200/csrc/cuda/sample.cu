@@ -422,8 +422,9 @@ __device__ uint32_t key_search(Shared& sm, Cluster& cl, const S& row, const Expo
       // the keys that the bin can hold: a hundredth of a bin more on either side, far above the rounding of bin_of
       bin = j;
       const float z_lo = ex.z_max - (j + 0.51f) / per, z_hi = ex.z_max - (j - 0.51f) / per;
-      if (per < 1e30f && z_lo > ex.z_cut && j < kBins - 1) lo = order_key(z_lo);
-      if (per < 1e30f && z_hi < ex.z_max) hi = order_key(z_hi);
+      const bool narrow = per > 0.0f && per < 1e30f;
+      if (narrow && z_lo > ex.z_cut && j < kBins - 1) lo = order_key(z_lo);
+      if (narrow && z_hi < ex.z_max) hi = order_key(z_hi);
     } else {
       const uint32_t new_hi = hi - (static_cast<uint32_t>(j) << shift);
       const u64 span = (1ull << shift) - 1;
@@ -528,7 +529,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
   int log_v = 0;
   while ((1ll << log_v) < a.vocab) ++log_v;
   ex.fraction = min(46, 62 - log_v);
-  ex.z_cut = fmaxf(zmax - kReach * t, -3.402823466e38f);   // -infinity has no mass at any temperature
+  // -infinity has no mass at any temperature, and neither has anything beside +infinity
+  ex.z_cut = zmax == CUDART_INF_F ? zmax : fmaxf(zmax - kReach * t, -3.402823466e38f);
   const double u = fmax(static_cast<double>(a.u[r]), 0.0), want_p = static_cast<double>(top_p);
   const double pmin = static_cast<double>(min_p) * static_cast<double>(ex.one());   // in units of mass
   const bool nucleus = top_p < 1.0f, filtered = k < a.vocab || nucleus || min_p > 0.0f;
@@ -539,8 +541,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
   if (filtered) {
     const float width = fminf(zmax - zmin, kReach * t);
     const float per = width > 0.0f ? fminf(static_cast<float>(kBins) / width, 1e37f) : 0.0f;
-    // the nearest whole number to (zmax - z) * per, left in the low bits by adding 2^23
-    auto bin_of = [&](float z) { return min(__float_as_int(fmaf(zmax - z, per, 8388608.0f)) & 0x7fffff, kBins - 1); };
+    // the nearest whole number to (zmax - z) * per, left in the low bits by adding 2^23. A difference that overflows goes to the last
+    // bin (as NaN where `per` is 0: fminf takes the other operand).
+    auto bin_of = [&](float z) { return __float_as_int(fminf(fmaf(zmax - z, per, 8388608.0f), 8388608.0f + (kBins - 1))) & 0x7fffff; };
     row.each(ex.z_cut, [&](int, float z) { atomicAdd(&sm.count[bin_of(z)], 1u); });
     cl.sync();
     u64 x[kPerThread], total;
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
 
     if (n_cut <= kList) {
       // ---- the short way, in the first CTA: candidates go to their bin's places, are ranked inside it, and decided on
-      const float z_lo = bin_cut < kBins - 1 && per < 1e30f ? fmaxf(zmax - (bin_cut + 0.51f) / per, ex.z_cut) : ex.z_cut;
+      const float z_lo = bin_cut < kBins - 1 && per > 0.0f && per < 1e30f ? fmaxf(zmax - (bin_cut + 0.51f) / per, ex.z_cut) : ex.z_cut;
       row.each(z_lo, [&](int i, float z) {
         if (bin_of(z) > bin_cut) return;
         sm.list[atomicAdd(&sm.n, 1u)] = (static_cast<u64>(order_key(z)) << 32) | static_cast<uint32_t>(~(row.first + i));
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
     }
 
     // ---- the long way: thresholds by histograms of counts and masses
-    if (bin_m < kBins - 1 && per < 1e37f) floor = fmaxf(floor, zmax - (bin_m + 0.51f) / per);   // min_p keeps nothing below
+    if (bin_m < kBins - 1 && per > 0.0f && per < 1e37f) floor = fmaxf(floor, zmax - (bin_m + 0.51f) / per);   // min_p keeps nothing below
     if (above_k < static_cast<u64>(k) && total > static_cast<u64>(k)) {
       const uint32_t key = key_search(sm, cl, row, ex, bin_of, per, static_cast<double>(k), [](int, float, uint32_t) { return true; },
                                       [](float) { return 1ull; });
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_rows_kernel(const SampleAr
         __syncthreads();
         // the bin's elements, ranked in the first CTA: the last one with less than `want` before it is the last to be kept
         if (j >= 0) {
-          const bool narrow = per < 1e30f;   // (bounds a hundredth of a bin wide of it)
+          const bool narrow = per > 0.0f && per < 1e30f;   // (bounds a hundredth of a bin wide of it)
           const float z_lo = narrow && j < kBins - 1 ? fmaxf(zmax - (j + 0.51f) / per, ex.z_cut) : ex.z_cut;
           const float z_hi = narrow && j > 0 ? zmax - (j - 0.51f) / per : zmax;
           row.each(z_lo, [&](int i, float z) {
