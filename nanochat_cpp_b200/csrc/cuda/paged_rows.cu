@@ -708,7 +708,7 @@ PagedPlan paged_rows_plan(const PagedAttnArgs& a) {
   const long long want = 148LL * 16 * 3;
   const auto share = [&](long long runs) { return static_cast<long long>(std::ceil(static_cast<double>(keys) * units / runs)); };
   long long per = std::max(std::min<long long>(std::max<long long>(share(want), 64), 512), share(2 * want));
-  if (units >= want) per = keys;
+  if (units >= want) per = keys + 2 * kTile;   // (a window may touch one tile more)
   per = (std::min<long long>(std::max<long long>(per, kTile), 1 << 30) + kTile - 1) / kTile * kTile;
   PagedPlan p;
   p.split_keys = static_cast<int>(per);

@@ -19,7 +19,8 @@ def _peak(fn):
 
 
 @pytest.mark.parametrize("mx", [False, True])
-def test_workspace_does_not_grow_with_rows_times_table(mx):
+@pytest.mark.parametrize("window", [-1, 2000])
+def test_workspace_does_not_grow_with_rows_times_table(mx, window):
     """Many rows and a wide table, on pages that only this kernel takes: besides the output no more than half a gigabyte."""
     B, T, H, KV, D, page = 8, 2048, 32, 8, 128, 8
     table = torch.full((B, 2304), -1, dtype=torch.int32)
@@ -29,21 +30,22 @@ def test_workspace_does_not_grow_with_rows_times_table(mx):
     q = torch.zeros(B, T, H, D, dtype=torch.bfloat16, device="cuda")
     lens = torch.full((B,), 8, dtype=torch.int32, device="cuda")
     new = torch.full((B,), 5, dtype=torch.int32, device="cuda")
-    out, peak = _peak(lambda: ops.paged_chunk_attention(q, k, k, table.cuda(), lens, new, -1, None, s, s))
+    out, peak = _peak(lambda: ops.paged_chunk_attention(q, k, k, table.cuda(), lens, new, window, None, s, s))
     assert peak - out.numel() * 2 - table.numel() * 4 < (1 << 29) and not out.any()
     ops.cuda_module().check_status()
 
 
 @pytest.mark.parametrize("H,KV,T", [(8, 8, 1), (10, 10, 13), (32, 4, 4), (6, 2, 50)])
-def test_workspace_is_bounded_for_any_number_of_units(H, KV, T):
-    """Under 7104 units there are at most twice as many runs and one more per unit: 21312 runs of 32 rows of D + 2 numbers."""
+@pytest.mark.parametrize("window", [-1, 2000])
+def test_workspace_is_bounded_for_any_number_of_units(H, KV, T, window):
+    """Under 7104 units there are at most twice as many runs and two more per unit: 28416 runs of 32 rows of D + 2 numbers."""
     for B in (1, 33, 200):
         table = torch.full((B, 65536), -1, dtype=torch.int32, device="cuda")
         k = torch.zeros(1, 8, KV, 64, dtype=torch.bfloat16, device="cuda")
         q = torch.zeros(B, T, H, 64, dtype=torch.bfloat16, device="cuda")
         lens = torch.zeros(B, dtype=torch.int32, device="cuda")
-        out, peak = _peak(lambda: ops.paged_chunk_attention(q, k, k, table, lens))
-        assert peak <= 21312 * 32 * (64 + 2) * 4 + out.numel() * 2 + 4096 and not out.any()
+        out, peak = _peak(lambda: ops.paged_chunk_attention(q, k, k, table, lens, None, window))
+        assert peak <= 28416 * 32 * (64 + 2) * 4 + out.numel() * 2 + 4096 and not out.any()
 
 
 @pytest.mark.parametrize("mx", [False, True])
