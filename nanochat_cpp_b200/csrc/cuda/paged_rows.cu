@@ -46,6 +46,7 @@ constexpr int kStages = 3;       // ring depth per warp
 constexpr int kPart = 512;       // keys of a run whose page numbers are at hand, one per lane: a longer run goes part by part
 constexpr float kNoMax = -1.0e30f;
 constexpr int kReach = 14;       // powers of two from the largest scale to one that is a normal f16: its codes are exact there
+constexpr int kUnset = -1000;    // no reference yet: out of reach of every scale byte
 constexpr int kClimb = 45;       // that the scale of the values' sums may grow by before what was summed first would lose bits
 
 template <bool F16>
@@ -82,7 +83,8 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ float pow2(int d) { return __uint_as_float(static_cast<uint32_t>(min(max(127 + d, 0), 255)) << 23); }
+// 2^(b - 127) of a scale byte, or of kUnset (any finite number)
+__device__ __forceinline__ float scale_value(int b) { return __uint_as_float(b > 0 ? static_cast<uint32_t>(b) << 23 : 0x00400000u); }
 // 2^d for d <= 0 (0 below the range of fp32)
 __device__ __forceinline__ float pow2_neg(int d) { return __uint_as_float(static_cast<uint32_t>(max(127 + d, 0)) << 23); }
 // of each half the smaller magnitude (its sign means nothing)
@@ -231,7 +233,7 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
   // Codes enter the f16 products as code * 2^(b - ref): exact while b lies no more than kReach below ref, the largest scale
   // byte of the tile's usable keys or more (keys), of the run's usable values so far (values). The scores take 2^(k_ref - 127)
   // into their factor; a larger v_ref scales down what has been summed.
-  int k_ref = 0, v_ref = 0, v_first = 0;
+  int k_ref = kUnset, v_ref = kUnset, v_first = kUnset;
   float k_unit = 1.0f;
 
   uint8_t* ring = smem;
@@ -409,7 +411,7 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
           for (int j = 0; j < 4; ++j) uv[j] = bv[j] - (v_ref - kReach), most = max(most, uv[j]);
           if (__any_sync(0xffffffffu, most > static_cast<uint32_t>(kReach))) {
             // rare: other references. NaN (255: the codes are NaN already) and keys that are none count for nothing
-            int hk = 0, lk = 255, hv = 0, lv = 255;
+            int hk = kUnset, lk = 255, hv = kUnset, lv = 255;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               if (bk[j] == 255 || !key_ok(g8 + 8 * j)) bk[j] = -1;
@@ -422,14 +424,14 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
             }
             hk = __reduce_max_sync(0xffffffffu, hk), lk = __reduce_min_sync(0xffffffffu, lk);
             hv = __reduce_max_sync(0xffffffffu, hv), lv = __reduce_min_sync(0xffffffffu, lv);
-            hk = hk > 0 ? hk : k_ref, hv = max(hv, v_ref);
-            v_first = v_first > 0 ? v_first : hv;
+            hk = hk != kUnset ? hk : k_ref, hv = max(hv, v_ref);
+            v_first = v_first != kUnset ? v_first : hv;
             if (lk < hk - kReach || lv < hv - kReach || hv - v_first > kClimb) {   // too far apart for f16
               copy_wait<0>();
               __syncwarp();
               return false;
             }
-            k_ref = hk, k_unit = __uint_as_float(static_cast<uint32_t>(k_ref) << 23);
+            k_ref = hk, k_unit = scale_value(k_ref);
             const float alpha = pow2_neg(v_ref - hv);
             v_ref = hv;
 #pragma unroll
@@ -600,7 +602,7 @@ __device__ __forceinline__ bool walk(const PagedAttnArgs& a, uint8_t* smem) {
 
   // ---- the run's result: rows 2c, 2c + 1 of every eight, channels g8 * D/8 + x
   const bool whole = rg.tiles <= split_tiles;   // no other run has keys: the result is final
-  const float unit = F16 ? pow2(v_ref - 127) : 1.0f;
+  const float unit = F16 ? scale_value(v_ref) : 1.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

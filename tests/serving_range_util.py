@@ -37,7 +37,8 @@ def expect(c, window=-1, scale=None, exact_products=False):
     rounding the probabilities moves the quotient by u (A + |o|), rounding the result by u |o|. An error d_j of score j, however,
     counts with its own weight: sum_j w_j d_j (|v_j| + |o|), so that a key of enormous size and no weight does not
     loosen the bound. d_j = (D + 2) 2^-24 |scale| sum |q_i k_ji| + 2^-21 for fp32 sums of products and the exponential; where all
-    products and sums are whole numbers below 2^24 only the scaling rounds: 4 * 2^-24 |s_j| + 2^-21. 1 % for second order."""
+    products and sums are whole numbers below 2^24 only the scaling rounds: 4 * 2^-24 |s_j| + 2^-21. 1 % for second order. Below 2^-126
+    bf16 steps by 2^-133: half a step for the values and half for the result are added."""
     q, B, T, H, D = c["q"].double(), *c["q"].shape
     k, v = U.pool_values(c["k"], c["ks"]), U.pool_values(c["v"], c["vs"])
     KV, page = k.shape[2], k.shape[1]
@@ -69,7 +70,7 @@ def expect(c, window=-1, scale=None, exact_products=False):
             o, A = w @ vh, w @ vh.abs()
             wd = torch.where(w > 0, w * d, torch.zeros_like(w))
             out[b, :n, h] = o
-            bound[b, :n, h] = 1.01 * (u * A + 2 * u * o.abs() + wd @ vh.abs() + wd.sum(-1, keepdim=True) * o.abs())
+            bound[b, :n, h] = 1.01 * (u * A + 2 * u * o.abs() + wd @ vh.abs() + wd.sum(-1, keepdim=True) * o.abs()) + 2.0 ** -133
     return out, bound
 
 

@@ -94,3 +94,20 @@ def test_infinities_and_nan_that_are_seen(variant):
                 elif what != what:
                     assert bool(out[0, 0, 0].isnan().all())
     ops.cuda_module().check_status()
+
+
+@pytest.mark.parametrize("variant,kb,vb", [(ROWS, 0, 0), (ROWS, 0, 127)] +
+                         [(v, kb, vb) for v in (ROWS, CHUNK) for kb, vb in ((127, 0), (5, 5), (100, 200), (220, 5))])
+@pytest.mark.parametrize("D,page,T", [(128, 16, 1), (64, 48, 3), (64, 32, 20)])
+def test_scale_bytes_at_the_ends(variant, D, page, T, kb, vb):
+    """Pools that a program filled itself: any byte but 255 is a power of two. The queries bring the scores back to order one. (The
+    many-rows kernel makes bf16 of a key, which holds every code from byte 3 on.)"""
+    g = torch.Generator().manual_seed(kb + vb)
+    B, H, KV, S = 2, 4, 2, 90
+    q = R.unit(g, B, T, H, D) * 2.0 ** (127 - max(kb, 10))
+    c = R.case(q, R.unit(g, B, S, KV, D), torch.randn(B, S, KV, D, generator=g), [S, 50], True, page=page)
+    for n, b in (("k", kb), ("v", vb)):
+        c[n + "s"] += b - 120                      # blocks of order one have a byte of 119 to 121
+        if b == 0:
+            c[n + "s"].zero_()
+    R.hold(c, variant)
