@@ -791,6 +791,8 @@ def generate_multi(engine: InferenceEngine, prompts, params: GenerateParams,
         if not bool(live.any()):
             break
         host_nxt, host_live = nxt.tolist(), live.tolist()
+        if on_device and any(t < 0 and alive for t, alive in zip(host_nxt, host_live)):
+            raise ValueError("generate: a row of logits holds no number above -infinity")
         for r in range(rows):
             if host_live[r]:
                 out[r].tokens.append(host_nxt[r])
