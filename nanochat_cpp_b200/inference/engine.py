@@ -298,6 +298,8 @@ class _CacheRows:
     def append_floor(self, new_len: int) -> int:
         return self.parent.append_floor(new_len)
 
+    append = PagedKVCache.append
+
     def advance_host(self, count: int, rows=None) -> None:
         self.parent.advance_host(count, self.index)
         self.lens_host = [n + count for n in self.lens_host]
