@@ -487,7 +487,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       auto probabilities = [&](int piece) {
         if (far) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sv[e] -= m_ref;
+          for (int e = 0; e < 32; e += 2) unpack2(add2(pack2(sv[e], sv[e + 1]), pack2(-m_ref, -m_ref)), sv[e], sv[e + 1]);
         }
         const float off = far ? 0.0f : -m_ref * sl;
         const uint64_t sl2 = pack2(sl, sl), m2 = pack2(off, off);
