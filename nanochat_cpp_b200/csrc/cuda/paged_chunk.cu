@@ -18,7 +18,9 @@
 // (a place behind the sequence's end) may be NaN, and 0 * NaN is not 0.
 // The running maximum is raised only when a tile exceeds it by more than 2^8: then the thread rescales its O row in tensor
 // memory. Bounds, per 128 x 128 tile: 1024 clocks for the exponentials (16 a clock and SM), 1024 for the two products.
-// Measured (B200, D = 128): 2 x 2048 over 18k keys 386 us on bf16 pages (866 TFLOP/s), 482 on MXFP8 (693); 8 ragged
+// Probabilities are rounded to bf16, the tensor core's operand type of V's range; the row's sum takes them unrounded, in fp32 (each
+// probability is off by 2^-8 of itself at most, in either direction).
+// Measured (B200, D = 128): 2 x 2048 over 18k keys 387 us on bf16 pages (865 TFLOP/s), 482 on MXFP8 (694); 8 ragged
 // prompts up to 2048, window 1024, 93 us.
 // grid: (blocks of 256 rows x key runs, kv heads x head packs, sequences), the blocks that see most first.
 #include <cuda.h>
@@ -706,9 +708,12 @@ bool paged_chunk_can(const PagedAttnArgs& a) {
 }
 
 bool paged_chunk_takes(const PagedAttnArgs& a) {
-  // Few rows per kv head leave most of a 128-row tile empty, and the other kernel reads the keys at full speed. Little work
-  // in all is done before this kernel has started up: up to some 1.5 GFLOP (as many as the page table has room for) the
-  // other is faster (3 x 77 tokens, 4 heads of 64, 777 keys: 14 against 25 us).
+  // Few rows per kv head leave most of a 128-row tile empty, and the other kernel reads the keys at full speed: 16 sequences,
+  // 4 kv heads, 4000 keys of 128 channels, other / this kernel: 16 rows 53 / 66 us (bf16 pages), 49 / 75 (MXFP8), 20 rows 83 / 68 and
+  // 76 / 78, 32 rows 96 / 70 and 88 / 80. (Of 64 channels they meet between 32 and 64 rows: at 32, 49 / 59 and 57 / 68.)
+  // Little work in all is done before this kernel has started up. The rule of 1.5 GFLOP, counted over the page table's width because a
+  // captured call knows no lengths, is coarse: 3 x 77 tokens, 4 heads of 64: 777 keys (0.2 GFLOP) 19 / 25 us, 3077 keys (0.7) 31 / 26;
+  // 1 x 200, 8 heads of 128: 200 keys (0.2) 23 / 16, 1000 keys (0.8) 27 / 31, 2200 keys (1.8) 49 / 31.
   double keys = static_cast<double>(a.max_pages) * a.page_size;
   if (a.window_left >= 0) keys = std::min(keys, static_cast<double>(a.window_left) + 1 + a.T);
   return a.T * (a.H / a.KV) > 16 && 4.0 * a.D * a.H * a.T * a.B * keys > 1.5e9 && paged_chunk_can(a);

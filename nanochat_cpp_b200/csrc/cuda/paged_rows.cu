@@ -18,9 +18,10 @@
 // score exceeds it by 2^8 or 2^7 (exact after the division by the sum), so the usual tile needs one vote and no shuffles.
 // Probabilities are rounded to 16 bits for the second product; the sum is taken of the rounded values, in fp32. On MXFP8 pages
 // the products run in f16, which takes E4M3 codes in one instruction a pair and probabilities to 11 bits (and to 2^-32 of the
-// reference). A run whose blocks, or whose queries' channels, lie further apart than f16 reaches is walked again in bf16.
-// Measured (B200, MXFP8, D = 128): 64 sequences up to 2048 keys 50 us (3.45 TB/s), 32 up to 32768 172..181 us (4.9 TB/s);
-// 64 x 4 new tokens over bf16 70 us (4.9 TB/s).
+// reference). A run whose blocks, or whose queries' channels, lie further apart than f16 reaches is walked again in bf16: where all
+// are, 64 sequences of 2000 keys take 121 us instead of 88, 32 of 20000 236 instead of 172.
+// Measured (B200, MXFP8, D = 128): 64 sequences up to 2048 keys 50..51 us (3.4 TB/s), 32 up to 32768 173..181 us (4.9..5.1 TB/s);
+// 64 x 4 new tokens over bf16 71 us (4.9 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>

@@ -581,7 +581,8 @@ class InferenceEngine:
     def extend(self, cache: PagedKVCache, tokens: torch.Tensor, counts: Optional[Sequence[int]] = None,
                all_logits: bool = False) -> torch.Tensor:
         """Append the first counts[b] (default: all) of tokens [B, T] to sequence b, each sequence at its own position:
-        prompts of different lengths, a further turn of a conversation, drafted tokens to verify. Returns the logits of
+        prompts of different lengths, a further turn of a conversation, drafted tokens to score (the cache keeps them all:
+        it can forget a sequence, not its last tokens). Returns the logits of
         every sequence's last new token [B, vocab] (zeros where counts[b] is 0) or, with `all_logits`, those of all new
         tokens [B, T, vocab] (zeros behind counts[b]). Longer inputs than the cache's windowed layers hold at once
         go through in pieces."""

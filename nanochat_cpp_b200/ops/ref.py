@@ -750,7 +750,9 @@ def paged_chunk_attention(q, k_pool, v_pool, page_table, seq_lens, q_lens=None, 
     the first q_lens[b] (None: T) rows of sequence b are its last q_lens[b] positions of seq_lens[b]. Row t sees keys
     j <= its position p = seq_lens[b] - q_lens[b] + t with p - j <= window_left. With `k_scale` / `v_scale` the pools
     are MXFP8 (see `kv_append_mx`), without them they have the type of q. The kernels take D = 64 or 128. Rows at or behind q_lens[b] and rows that
-    see no key are zero. A key past the page table or on a page outside the pool is left out."""
+    see no key are zero. A key past the page table or on a page outside the pool is left out.
+    A value that is not finite and that some row of a sequence sees may reach all rows of that sequence and head (0 * NaN); keys that
+    no row sees do not count. Sums of probability times value are fp32: values up to 2^90 in magnitude cannot overflow them."""
     name = "paged_chunk_attention"
     _check(q.dim() == 4 and q.stride(3) == 1, f"{name}: q must be [B, T, H, D] with dense channels")
     B, T, H, D = q.shape
