@@ -111,3 +111,17 @@ def test_scale_bytes_at_the_ends(variant, D, page, T, kb, vb):
         if b == 0:
             c[n + "s"].zero_()
     R.hold(c, variant)
+
+
+@pytest.mark.parametrize("variant", [ROWS, CHUNK])
+@pytest.mark.parametrize("size,key_size", [(0.0, 1.0), (2.0 ** -125, 2.0 ** 115), (2.0 ** -132, 2.0 ** 118), (2.0 ** 110, 2.0 ** -110), (2.0 ** 60, 2.0 ** -90)])
+@pytest.mark.parametrize("T", [1, 9])
+def test_queries_of_any_size(variant, size, key_size, T):
+    """Zeros (every key weighs the same), numbers below bf16's normal range and large ones, some channels zero."""
+    g = torch.Generator().manual_seed(5)
+    B, H, KV, D, S = 2, 4, 2, 128, 300
+    q = R.unit(g, B, T, H, D) * size
+    q[..., 3::7] = 0
+    q[0, 0, 0] = 0
+    R.hold(R.case(q, R.unit(g, B, S, KV, D) * key_size, torch.randn(B, S, KV, D, generator=g), [S, S - 100], True), variant)
+    R.hold(R.case(q, R.unit(g, B, S, KV, D) * key_size, torch.randn(B, S, KV, D, generator=g), [S, S - 100], False), variant)
