@@ -618,7 +618,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               *reinterpret_cast<uint4*>(dst + c * 32 + g * 4) = make_uint4(w[g * 4], w[g * 4 + 1], w[g * 4 + 2], w[g * 4 + 3]);
           }
         }
-        if (row_in && half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref * sl, any ? l_run : 0.0f);
+        // (the reference before the scale: the difference of two is exact where their products with it are not)
+        if (row_in && half == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref, any ? l_run : 0.0f);
       }
     }
   }
@@ -672,7 +673,7 @@ const char* launch_chunk(const PagedAttnArgs& args, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(blocks) * args.splits, p.a.KV, args.B);
   paged_chunk_kernel<D, MX><<<grid, L::kThreads, L::kTotal, s>>>(tq, tk, tv, p);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && args.splits > 1) e = launch_combine<D>(p.a, NQ * BQ, BKV, s);
+  if (e == cudaSuccess && args.splits > 1) e = launch_combine<D>(p.a, NQ * BQ, BKV, args.scale * 1.4426950408889634f, s);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 

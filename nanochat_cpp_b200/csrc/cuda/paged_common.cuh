@@ -50,10 +50,10 @@ __device__ __forceinline__ Range range_of(const PagedAttnArgs& a, int b, int r0,
   return g;
 }
 
-// out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the runs of a row; rows that one run finished are skipped.
+// out = sum_s o_s 2^(unit (m_s - M)) / sum_s l_s 2^(unit (m_s - M)) over the runs of a row; rows that one run finished are skipped.
 // WARPS warps share a row (many runs, few rows), or each of the CTA's four warps takes a row (WARPS = 1).
 template <int D, int WARPS>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a, int rows, int tile) {
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a, int rows, int tile, float unit) {
   constexpr int ROWS_HERE = 4 / WARPS;
   __shared__ float sm_o[4][D], sm_l[4], sm_m[4];
   NC_PDL_PROLOGUE();
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
   for (int s = part; s < n; s += WARPS) {
     const long long p = at + static_cast<long long>(s) * rw;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
-    const float w = ml.y == 0.0f ? 0.0f : fast_exp2(ml.x - mx);   // a run that the row saw nothing of
+    const float w = ml.y == 0.0f ? 0.0f : fast_exp2((ml.x - mx) * unit);   // a run that the row saw nothing of
     ls = fmaf(w, ml.y, ls);
     if constexpr (E == 4) {
       const float4 x = *reinterpret_cast<const float4*>(a.part_o + p * D + lane * 4);
@@ -128,11 +128,11 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs 
 
 // Always launched behind the first kernel's tail (it waits for that kernel before it reads anything).
 template <int D>
-cudaError_t launch_combine(const PagedAttnArgs& a, int rows, int tile, cudaStream_t s) {
+cudaError_t launch_combine(const PagedAttnArgs& a, int rows, int tile, float unit, cudaStream_t s) {
   const long long total = static_cast<long long>(a.B) * a.T * a.H;
   if (total <= 2048)   // few rows: more loads in flight for each
-    return launch_pdl(true, paged_combine_kernel<D, 4>, dim3(static_cast<unsigned>(total)), dim3(128), 0, s, a, rows, tile);
-  return launch_pdl(true, paged_combine_kernel<D, 1>, dim3(static_cast<unsigned>((total + 3) / 4)), dim3(128), 0, s, a, rows, tile);
+    return launch_pdl(true, paged_combine_kernel<D, 4>, dim3(static_cast<unsigned>(total)), dim3(128), 0, s, a, rows, tile, unit);
+  return launch_pdl(true, paged_combine_kernel<D, 1>, dim3(static_cast<unsigned>((total + 3) / 4)), dim3(128), 0, s, a, rows, tile, unit);
 }
 
 }  // namespace

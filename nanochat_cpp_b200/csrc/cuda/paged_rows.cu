@@ -678,7 +678,7 @@ cudaError_t launch_rows(const PagedAttnArgs& a, cudaStream_t s) {
   cudaError_t e = launch_maybe_pdl(paged_rows_kernel<D, MX, NT, P16>, dim3(a.splits, a.KV * blocks, a.B), dim3(32), R::kBytes, s, a);
   if (e != cudaSuccess || a.splits <= 1) return e;
   // always behind the first kernel's tail (it waits for it before it reads anything)
-  return launch_combine<D>(a, ROWS, kTile, s);
+  return launch_combine<D>(a, ROWS, kTile, 1.0f, s);
 }
 template <int D, bool MX>
 cudaError_t launch_shape(const PagedAttnArgs& a, cudaStream_t s) {

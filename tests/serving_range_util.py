@@ -32,13 +32,13 @@ def case(q, k, v, lens, mx, q_lens=None, page=PAGE, width=None):
     return c
 
 
-def expect(c, window=-1, scale=None, exact_products=False):
+def expect(c, window=-1, scale=None, exact_products=False, score_error=None):
     """(result, bound) in 64 bits. As in `serving_util.attention`, with u = 2^-8 for a rounding to bf16 and A = sum w_j |v_j|:
     rounding the probabilities moves the quotient by u (A + |o|), rounding the result by u |o|. An error d_j of score j, however,
     counts with its own weight: sum_j w_j d_j (|v_j| + |o|), so that a key of enormous size and no weight does not
     loosen the bound. d_j = (D + 2) 2^-24 |scale| sum |q_i k_ji| + 2^-21 for fp32 sums of products and the exponential; where all
     products and sums are whole numbers below 2^24 only the scaling rounds: 4 * 2^-24 |s_j| + 2^-21. 1 % for second order. Below 2^-126
-    bf16 steps by 2^-133: half a step for the values and half for the result are added."""
+    bf16 steps by 2^-133: half a step for the values and half for the result are added. `score_error`: another d_j."""
     q, B, T, H, D = c["q"].double(), *c["q"].shape
     k, v = U.pool_values(c["k"], c["ks"]), U.pool_values(c["v"], c["vs"])
     KV, page = k.shape[2], k.shape[1]
@@ -63,7 +63,9 @@ def expect(c, window=-1, scale=None, exact_products=False):
             s = qh @ kh.T * scale
             w = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
             w = torch.where(some[:, None], w, torch.zeros_like(w))
-            if exact_products:
+            if score_error is not None:
+                d = torch.full_like(s, score_error)
+            elif exact_products:
                 d = 4 * 2.0 ** -24 * s.abs() + 2.0 ** -21
             else:
                 d = (D + 2) * 2.0 ** -24 * (qh.abs() @ kh.abs().T) * abs(scale) + 2.0 ** -21
@@ -84,9 +86,9 @@ def run(c, variant, window=-1, scale=None):
                                                    c["ks"], c["vs"], variant)
 
 
-def hold(c, variant, window=-1, scale=None, exact_products=False):
+def hold(c, variant, window=-1, scale=None, exact_products=False, score_error=None):
     out = run(c, variant, window, scale)
-    want, bound = expect(c, window, scale, exact_products)
+    want, bound = expect(c, window, scale, exact_products, score_error)
     bad = ~((out.double() - want).abs() <= bound)
     assert not bool(bad.any()), (int(bad.sum()), bad.numel(), bad.nonzero()[0].tolist(), float(out[bad][0]), float(want[bad][0]))
     ops.cuda_module().check_status()

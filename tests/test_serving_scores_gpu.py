@@ -69,3 +69,21 @@ def test_scores_where_fp32_steps_by_eight(variant, mx):
     low, high = values[:n].mean(0), values[n:].mean(0)
     assert bool(((out - (low + 256 * high) / 257).abs() <= 1.01 * 2.0 ** -7 * values.abs().mean(0) * 2).all())
     ops.cuda_module().check_status()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("S,T", [(400, 40), (3000, 40), (3000, 1)])
+def test_near_scores_of_large_size(mx, S, T):
+    """Whole-number scores of 7.3 million to three more in the many-rows kernel, whose differences matter: they are taken before the
+    scale, inside a run of keys and where runs are joined, so that only the first tiles' reference is rounded (a score may be
+    off by 2^-13)."""
+    g = torch.Generator().manual_seed(S)
+    q = torch.full((2, T, 2, 128), 240.0)
+    k = torch.full((2, S, 2, 128), 240.0)
+    q[..., 0] = 1
+    k[..., 0] = torch.randint(0, 3, (2, S, 2), generator=g).float()
+    k[:, S // 2:S // 2 + S // 8, :, 0] = 3          # the largest lie in one or two runs
+    v = torch.randn(2, S, 2, 128, generator=g).abs()
+    v[:, S // 2:S // 2 + S // 8] *= -1              # what the runs weigh shows
+    c = R.case(q, k, v, [S, S - 7], mx)
+    R.hold(c, CHUNK, scale=1.0, score_error=2.0 ** -13)
